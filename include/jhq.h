@@ -250,6 +250,76 @@ int jhq_sharded_search(jhq_sharded* idx, const float* q, int64_t nq, int k, floa
 int jhq_sharded_set_nprobe(jhq_sharded* idx, int nprobe);
 int64_t jhq_sharded_ntotal(const jhq_sharded* idx);
 
+/* ---- 8-bit rows --------------------------------------------------------
+ * The operators in front of add() and search() when the vectors come from an
+ * encoder model: the norm that ends its last layer, written as 8-bit rows; the
+ * product of such rows with an 8-bit projection, which gives the embeddings;
+ * and a cache that rows (keys, values, token vectors) are written to in 8 bits
+ * and read back from. No reference counterpart.
+ *
+ * An 8-bit row is a row of int8 values q[j] in -127..127, cut into `groups`
+ * equal groups with one float32 scale each; it stands for scale * q[j].
+ * Quantising the values y of a group: a = max |y|, q = rint(y * (127 *
+ * (1 / a))) (ties to even), scale = a / 127, all in float32. A group of zeros has scale 0
+ * and q = 0; a group that holds an infinity or a NaN has scale NaN and q = 0.
+ *
+ * All buffers are device memory of the current device; the calls are
+ * asynchronous on `stream` (cudaStream_t, NULL = the default stream), allocate
+ * nothing, keep nothing between calls and may be captured in a CUDA graph.
+ * Rows are `ld` elements apart, with any ld >= the row's length; base addresses
+ * must be multiples of the element's size. Rows that begin on 16-byte
+ * boundaries are fastest. rows = 0 is a call that does nothing. Bad arguments
+ * return JHQ_EINVAL before anything is launched. */
+#define JHQ_F32  0
+#define JHQ_F16  1
+#define JHQ_BF16 2
+typedef struct jhq_view {      /* a matrix of floating-point rows */
+    void*   data;
+    int64_t rows, cols;
+    int64_t ld;                /* elements from one row to the next */
+    int     type;              /* JHQ_F32, JHQ_F16 or JHQ_BF16 */
+} jhq_view;
+typedef struct jhq_q8_rows {   /* a matrix of 8-bit rows */
+    int8_t* q;                 /* [rows][dim], rows ld bytes apart */
+    float*  scale;             /* [rows][groups], packed */
+    int64_t rows, dim;
+    int64_t ld;
+    int     groups;            /* divides dim; 1 = one scale a row */
+} jhq_q8_rows;
+
+/* RMS norm with the residual's addition and 8-bit output. For each row, in
+ * float32: h = x + residual (residual NULL: h = x), out = the 8-bit row of
+ * h * weight / sqrt(mean(h^2) + eps) (weight NULL: ones), and, where
+ * residual_out is given, h rounded once to its type. weight is 1 x cols, of
+ * x's type or JHQ_F32; residual and residual_out have the same type, x's or
+ * JHQ_F32, and may be the same buffer. out->groups must be 1. h is normed as
+ * it is summed, before it is rounded for residual_out; sums of squares that
+ * leave float32's range are formed again from scaled values. */
+int jhq_q8_rms_norm(const jhq_view* x, const jhq_view* residual, const jhq_view* weight, float eps,
+                    const jhq_view* residual_out, const jhq_q8_rows* out, void* stream);
+
+/* out[t][n] = (sum_k x.q[t][k] * w.q[n][k]) * x.scale[t] * w.scale[n] + bias[n]:
+ * the sum exact in 32-bit integers, the rest in float32, rounded once to out's
+ * type. bias (1 x w->rows, JHQ_F32) may be NULL. Both groups must be 1,
+ * x->dim = w->dim <= 131071 (the largest for which no sum of products of any
+ * int8 values overflows), out is x->rows by w->rows and overlaps no input. */
+int jhq_q8_matmul(const jhq_q8_rows* x, const jhq_q8_rows* w, const jhq_view* bias,
+                  const jhq_view* out, void* stream);
+
+/* Writes row i of x, quantised, to row slots[i] of the cache (slots NULL: row
+ * i; x->rows <= cache->rows then). A slot outside [0, cache->rows) is skipped:
+ * padding is marked with -1. The other slots must differ from one another. */
+int jhq_q8_write(const jhq_view* x, const int64_t* slots, const jhq_q8_rows* cache, void* stream);
+/* Reads row slots[i] of the cache (slots NULL: row i) back into row i of out:
+ * scale * q in float32, rounded once to out's type. A slot outside
+ * [0, cache->rows) reads as zeros. */
+int jhq_q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out, void* stream);
+
+/* After the streams of the calls above have drained: JHQ_ETIMEDOUT (once) if a
+ * bounded device wait of one of them on the current device gave up, so that its
+ * output is not valid, else JHQ_OK. Synchronises with the device. */
+int jhq_q8_status(void);
+
 /* ---- per-stage timing (the reference's jhq_v9_step_timing / v13 step
  * events, jhq_v13_step_timing/search.cu:456-491) -------------------------
  * With profiling on, search runs each batch as direct launches (no CUDA

@@ -41,7 +41,8 @@ EXPORTED = [
     "jhq_probe_device",
     "jhq_search_device_probes", "jhq_sharded_create", "jhq_sharded_destroy",
     "jhq_sharded_train", "jhq_sharded_add", "jhq_sharded_search", "jhq_sharded_set_nprobe",
-    "jhq_sharded_ntotal",
+    "jhq_sharded_ntotal", "jhq_q8_rms_norm", "jhq_q8_matmul", "jhq_q8_write", "jhq_q8_read",
+    "jhq_q8_status",
 ]
 STAGES = ["rotate", "coarse+probes", "plan", "scan", "refine"]
 
@@ -145,6 +146,7 @@ def load_library(path: str = "") -> C.CDLL:
     L.jhq_kernel_launches.restype = C.c_int64
     L.jhq_last_error.restype = C.c_char_p
     L.jhq_version.restype = C.c_char_p
+    q8._declare(L)
     _lib = L
     return L
 
@@ -499,3 +501,8 @@ class JHQShardedIndex:
         _check(self._L.jhq_sharded_search(self._h, _ptr(q, C.c_float), nq, k, _ptr(D, C.c_float),
                                           _ptr(I, C.c_int32)))
         return D, I
+
+
+from . import q8  # noqa: E402  (uses load_library and _check above)
+from .q8 import (Q8Rows, View, q8_check_status, q8_matmul, q8_read, q8_rms_norm,  # noqa: E402,F401
+                 q8_write)

@@ -14,6 +14,7 @@
 #include "index.h"
 #include "sharded.h"
 #include "kernels.cuh"
+#include "q8.h"
 #include "train_cpu.h"
 
 struct jhq_index {
@@ -282,6 +283,32 @@ int jhq_merge_shards(const float* d_in_dists, const int32_t* d_in_ids, int nshar
             jhq::fail(JHQ_EINVAL, "merge_shards: null buffer");
         jhq::merge_shard_lists(d_in_dists, d_in_ids, nshards, nq, k, d_out_dists, d_out_ids,
                                static_cast<cudaStream_t>(stream));
+    });
+}
+
+int jhq_q8_rms_norm(const jhq_view* x, const jhq_view* residual, const jhq_view* weight, float eps,
+                    const jhq_view* residual_out, const jhq_q8_rows* out, void* stream) {
+    return guarded([&] {
+        jhq::q8_rms_norm(x, residual, weight, eps, residual_out, out, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int jhq_q8_matmul(const jhq_q8_rows* x, const jhq_q8_rows* w, const jhq_view* bias,
+                  const jhq_view* out, void* stream) {
+    return guarded([&] { jhq::q8_matmul(x, w, bias, out, static_cast<cudaStream_t>(stream)); });
+}
+
+int jhq_q8_write(const jhq_view* x, const int64_t* slots, const jhq_q8_rows* cache, void* stream) {
+    return guarded([&] { jhq::q8_write(x, slots, cache, static_cast<cudaStream_t>(stream)); });
+}
+
+int jhq_q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out, void* stream) {
+    return guarded([&] { jhq::q8_read(cache, slots, out, static_cast<cudaStream_t>(stream)); });
+}
+
+int jhq_q8_status(void) {
+    return guarded([&] {
+        if (jhq::q8_take_error()) jhq::fail(JHQ_ETIMEDOUT, "a bounded device wait of an 8-bit product gave up");
     });
 }
 

@@ -1,0 +1,100 @@
+"""8-bit rows (jhq_q8_* of include/jhq.h): the RMS norm that ends an encoder layer and writes 8-bit rows, their
+product with an 8-bit projection, and a cache that rows are written to in 8 bits and read back from.
+
+    rows = Q8Rows.of(q, scale)                       # q: (n, d) int8, scale: (n,) float32, both on the GPU
+    q8_rms_norm(View.of(x), rows, weight=View.of(w), residual=View.of(r), residual_out=View.of(r))
+    q8_matmul(rows, Q8Rows.of(wq, w_scale), View.of(out))
+
+A View or Q8Rows describes device memory and does not keep it alive; `of` takes any 2-D tensor with data_ptr(),
+shape, stride() and dtype, such as torch's. Calls are asynchronous on `stream` (a raw CUDA stream, as
+torch.cuda.current_stream().cuda_stream) on the current device; errors are those of the package.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import jhq_gpu_b200 as _J
+
+F32, F16, BF16 = range(3)
+_TYPES = {"float32": F32, "float16": F16, "bfloat16": BF16,
+          "torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
+
+def _shape(t, what: str):
+    """rows, columns and row stride of a 2-D (or, as one row, 1-D) tensor."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 1:
+        shape, stride = (1, shape[0]), (shape[0] * stride[0], stride[0])
+    if len(shape) != 2:
+        raise ValueError(f"{what}: a 2-D tensor is needed, got {len(shape)} dimensions")
+    rows, cols = shape
+    if cols > 1 and stride[1] != 1:
+        raise ValueError(f"{what}: the values of a row must follow one another (stride {stride[1]})")
+    return rows, cols, stride[0] if rows > 1 else cols
+
+
+class View(C.Structure):
+    """jhq_view: a matrix of floating-point rows in device memory."""
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64),
+                ("type", C.c_int)]
+
+    @classmethod
+    def of(cls, t) -> "View":
+        kind = _TYPES.get(str(t.dtype))
+        if kind is None:
+            raise ValueError(f"View: float32, float16 or bfloat16 is needed, got {t.dtype}")
+        rows, cols, ld = _shape(t, "View")
+        return cls(t.data_ptr(), rows, cols, ld, kind)
+
+
+class Q8Rows(C.Structure):
+    """jhq_q8_rows: a matrix of 8-bit rows in device memory, one float32 scale for each group of a row."""
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("rows", C.c_int64), ("dim", C.c_int64),
+                ("ld", C.c_int64), ("groups", C.c_int)]
+
+    @classmethod
+    def of(cls, q, scale, groups: int = 1) -> "Q8Rows":
+        """q: (rows, dim) int8; scale: rows * groups float32, packed."""
+        if str(q.dtype) not in ("torch.int8", "int8") or str(scale.dtype) not in ("torch.float32", "float32"):
+            raise ValueError(f"Q8Rows: int8 values and float32 scales are needed, got {q.dtype} and {scale.dtype}")
+        rows, dim, ld = _shape(q, "Q8Rows")
+        if scale.numel() != rows * groups or not scale.is_contiguous():
+            raise ValueError(f"Q8Rows: {rows} x {groups} packed scales are needed")
+        return cls(q.data_ptr(), scale.data_ptr(), rows, dim, ld, groups)
+
+
+def _declare(L: C.CDLL) -> None:
+    v, r, p = C.POINTER(View), C.POINTER(Q8Rows), C.c_void_p
+    L.jhq_q8_rms_norm.argtypes = [v, v, v, C.c_float, v, r, p]
+    L.jhq_q8_matmul.argtypes = [r, r, v, v, p]
+    L.jhq_q8_write.argtypes = [v, p, r, p]
+    L.jhq_q8_read.argtypes = [r, p, v, p]
+    L.jhq_q8_status.argtypes = []
+
+
+def q8_rms_norm(x: View, out: Q8Rows, weight: Optional[View] = None, residual: Optional[View] = None,
+                residual_out: Optional[View] = None, eps: float = 1e-6, stream: int = 0) -> None:
+    """out = 8-bit rows of h * weight / sqrt(mean(h^2) + eps), h = x + residual; residual_out = h."""
+    _J._check(_J.load_library().jhq_q8_rms_norm(x, residual, weight, eps, residual_out, out, stream))
+
+
+def q8_matmul(x: Q8Rows, w: Q8Rows, out: View, bias: Optional[View] = None, stream: int = 0) -> None:
+    """out[t][n] = (sum_k x.q[t][k] w.q[n][k]) * x.scale[t] * w.scale[n] + bias[n], the sum exact."""
+    _J._check(_J.load_library().jhq_q8_matmul(x, w, bias, out, stream))
+
+
+def q8_write(x: View, cache: Q8Rows, slots: Optional[int] = None, stream: int = 0) -> None:
+    """Row i of x, quantised, to row slots[i] of the cache (slots: a device pointer to int64s; None: row i).
+    Slots outside the cache (-1) are skipped."""
+    _J._check(_J.load_library().jhq_q8_write(x, slots, cache, stream))
+
+
+def q8_read(cache: Q8Rows, out: View, slots: Optional[int] = None, stream: int = 0) -> None:
+    """Row slots[i] of the cache into row i of out, as scale * q; slots outside the cache read as zeros."""
+    _J._check(_J.load_library().jhq_q8_read(cache, slots, out, stream))
+
+
+def q8_check_status() -> None:
+    """Raises JHQError (JHQ_ETIMEDOUT) if a device wait of these operators gave up; synchronises."""
+    _J._check(_J.load_library().jhq_q8_status())
