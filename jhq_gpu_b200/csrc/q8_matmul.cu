@@ -1,8 +1,22 @@
 // q8_matmul.cu — the product of two sets of 8-bit rows,
 //   out[t][n] = (sum_k x[t][k] w[n][k]) * sx[t] * sw[n] + bias[n],
-// the sum exact in 32-bit integers.
+// the sum exact in 32-bit integers on the tensor cores (tcgen05 kind::i8,
+// operands in 128-byte K blocks staged in a ring of shared memory, sums in TMEM).
+// Two kernels: panels (few tokens, where the weights' bytes count, or rows that
+// TMA cannot fetch) and pairs (many tokens, where the multiply-adds count).
+//
+// Every wait on an mbarrier is bounded (about a second); one that gives up sets
+// g_q8_error (jhq_q8_status) and the CTA's abort flag, which ends every role's
+// loop. Before it leaves, a CTA lets the copies and MMAs it issued finish (bounded
+// again) and frees its TMEM.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
 
 #include "kernels.cuh"
 #include "q8.h"
@@ -19,7 +33,12 @@ struct Epilogue {                   // what turns a sum into an output
     int64_t ldo;
     int64_t T;
     int N, type;
+    bool vec;                       // output rows begin on 16-byte boundaries
 };
+
+__device__ __forceinline__ void store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ void store_out(const Epilogue& e, int64_t t, int n, float v) {
     const int64_t at = t * e.ldo + n;
@@ -28,48 +47,737 @@ __device__ __forceinline__ void store_out(const Epilogue& e, int64_t t, int n, f
     else static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(v);
 }
 
-constexpr int TILE = 64, KC = 64;   // outputs a side, bytes of K a step
+constexpr long long WAIT_CYCLES = 1ll << 31;     // about a second
 
-// Any alignment: bytes are loaded one by one. 256 threads, 4 x 4 sums each.
-__global__ void __launch_bounds__(256)
-simple_kernel(const int8_t* __restrict__ x, int64_t ldx, const int8_t* __restrict__ w, int64_t ldw, int K,
-              Epilogue e) {
-    __shared__ int xs[TILE][KC / 4 + 1], ws[TILE][KC / 4 + 1];
-    const int64_t t0 = (int64_t)blockIdx.x * TILE;
-    const int n0 = blockIdx.y * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += KC) {
-        for (int i = threadIdx.x; i < TILE * KC; i += 256) {
-            const int r = i / KC, c = i % KC, k = k0 + c;
-            reinterpret_cast<int8_t*>(xs[r])[c] =
-                t0 + r < e.T && k < K ? x[(t0 + r) * ldx + k] : (int8_t)0;
-            reinterpret_cast<int8_t*>(ws[r])[c] =
-                n0 + r < e.N && k < K ? w[(int64_t)(n0 + r) * ldw + k] : (int8_t)0;
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
+// Bounded wait for the phase of parity `parity`; gives up when the CTA's abort
+// flag is set or after WAIT_CYCLES, which sets the flag and g_q8_error.
+__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    if (mbar_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (abort && *abort) return false;
+        if (clock64() - t0 > WAIT_CYCLES) {
+            atomicExch(&g_q8_error, 1);
+            if (abort) *abort = 1;
+            return false;
         }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < KC / 4; ++c) {
-            int a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { a[i] = xs[ty + 16 * i][c]; b[i] = ws[tx + 16 * i][c]; }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[i], b[j], acc[i][j]);
-        }
-        __syncthreads();
     }
+    return true;
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared address `a` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_to(uint32_t a, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+
+// One lane of a converged warp; unlike a test of the lane's number, the compiler
+// knows that a single thread goes on, and issues its MMAs and copies directly.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+// Stage and phase of a ring of N.
+template <int N>
+struct Ring {
+    int s = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == N) { s = 0; phase ^= 1u; }
+    }
+};
+
+// K-major operand with 128-byte swizzle: rows of 128 bytes, 8-row groups 1024
+// bytes apart, descriptor version 1, layout type 2.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+template <int CTAS>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    if (CTAS == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+            :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+            :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add));
+}
+// The MMAs of one K block of `left` bytes, 32 each.
+template <int CTAS>
+__device__ __forceinline__ void mma_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int left, bool add) {
+    if (left > 96) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < 4; ++k) mma_i8<CTAS>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : (uint32_t)add);
+    } else {
+        for (int k = 0; 32 * k < left; ++k) mma_i8<CTAS>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : (uint32_t)add);
+    }
+}
+// s32 sums of s8 operands, both K-major.
+constexpr uint32_t idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld16(int* r, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(int* r, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr) : "memory");
+}
+
+// 16 outputs of channel n, tokens t .. t + 15, from the sums in r; lane l holds
+// the scale of token t - at + l. Every lane of the warp calls it (n differs, t
+// does not).
+template <class O>
+__device__ __forceinline__ void put16(const Epilogue& e, const int* r, int64_t t, float sx, int at, int n, float sw, float b) {
+    const int left = (int)min((int64_t)16, e.T - t);
+    O* o = static_cast<O*>(e.out) + t * e.ldo + n;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t t = t0 + ty + 16 * i;
-            const int n = n0 + tx + 16 * j;
-            if (t < e.T && n < e.N) {
-                const float v = (float)acc[i][j] * e.sx[t] * e.sw[n];
-                store_out(e, t, n, e.bias ? v + e.bias[n] : v);
+    for (int j = 0; j < 16; ++j) {
+        const float v = (float)r[j] * __shfl_sync(~0u, sx, at + j) * sw;
+        if (j < left && n < e.N) store(o + j * e.ldo, e.bias ? v + b : v);
+    }
+}
+__device__ __forceinline__ void put16(const Epilogue& e, const int* r, int64_t t, float sx, int at, int n, float sw, float b) {
+    if (t >= e.T) return;
+    if (e.type == JHQ_BF16) put16<__nv_bfloat16>(e, r, t, sx, at, n, sw, b);
+    else if (e.type == JHQ_F16) put16<__half>(e, r, t, sx, at, n, sw, b);
+    else put16<float>(e, r, t, sx, at, n, sw, b);
+}
+// The scales of tokens t .. t + 32 COUNT - 1, 32 a register.
+template <int COUNT>
+__device__ __forceinline__ void get_scales(const Epilogue& e, int64_t t, float* sx) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const int64_t at = t + 32 * i + (threadIdx.x & 31);
+        sx[i] = at < e.T ? e.sx[at] : 0.0f;
+    }
+}
+// A warp's wait: lane 0 polls.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort);
+    return __all_sync(~0u, ok);
+}
+
+// ---- panels: few tokens, or rows at any address ------------------------------
+//
+// out^T = W x^T: a CTA takes 128 channels (the rows of the MMA) by TN tokens
+// (its columns) over one slice of K; the S CTAs of a cluster take the S slices
+// of one tile and add their sums through distributed shared memory, each
+// finishing TN / S of the tokens. 32-bit integer sums are exact, so the split
+// changes no output.
+constexpr int BM = 128, BK = 128;
+constexpr int LOADERS = 256;                               // threads that load where TMA cannot
+constexpr int panel_threads(bool tma) { return 64 + (tma ? 128 : LOADERS); }
+
+template <int TN>
+struct Panel {
+    static constexpr int STAGE = (BM + TN) * BK;
+    static constexpr int STAGES = TN == 16 ? 10 : TN == 32 ? 9 : TN == 64 ? 8 : 6;
+    static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+    static constexpr uint32_t COLS = TN < 32 ? 32 : TN;
+    static_assert(BM * TN * 4 <= STAGES * STAGE, "partial sums reuse the stages");
+};
+
+struct Rows8 {                       // operand rows for the loader threads
+    const int8_t* p;
+    int64_t ld, rows;
+};
+
+// One warp copies bytes k .. k + 127 of R rows (row0 + r0, + r0 + step, ...) into
+// swizzled 128-byte rows of shared memory, zeros beyond the rows' ends. Rows
+// begin at any address: a lane reads an aligned word and shifts it together with
+// its neighbour's (lane 31 reads one more). Only words that lie inside the row are
+// read whole; the bytes of those that straddle its ends are read one by one. The
+// loads of all R rows are in flight together.
+template <int R>
+__device__ __forceinline__ void load_rows(const Rows8& m, int64_t row0, int r0, int step, int k, int K, uint32_t dst,
+                                          int lane) {
+    uint32_t lo[R], ex[R];
+    int off[R];
+    const bool edge = k == 0 || k + BK + 4 > K;            // the block touches an end of its rows
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int64_t row = row0 + r0 + i * step;
+        const bool in = row < m.rows;
+        const int8_t* at = m.p + (in ? row : 0) * m.ld + k;
+        off[i] = (int)((uintptr_t)at & 3);
+        const int pos = k - off[i] + 4 * lane;             // of the word in the row
+        const int8_t* a = at - off[i] + 4 * lane;
+        lo[i] = in && pos >= 0 && pos + 4 <= K ? *reinterpret_cast<const uint32_t*>(a) : 0u;
+        ex[i] = in && lane == 31 && pos + 8 <= K ? *reinterpret_cast<const uint32_t*>(a + 4) : 0u;
+        if (edge) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const bool b0 = in && (pos < 0 || pos + 4 > K) && pos + c >= 0 && pos + c < K;
+                const bool b1 = in && lane == 31 && pos + 8 > K && pos + 4 + c < K;
+                const uint32_t v0 = b0 ? (uint32_t)(uint8_t)a[c] : 0u, v1 = b1 ? (uint32_t)(uint8_t)a[4 + c] : 0u;
+                lo[i] |= v0 << (8 * c);
+                ex[i] |= v1 << (8 * c);
             }
         }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        uint32_t hi = __shfl_down_sync(~0u, lo[i], 1);
+        if (lane == 31) hi = ex[i];
+        const int r = r0 + i * step;
+        asm volatile("st.shared.b32 [%0], %1;"
+                     :: "r"(dst + r * 128 + ((4 * lane) ^ ((r & 7) << 4))), "r"(__funnelshift_r(lo[i], hi, 8 * off[i]))
+                     : "memory");
+    }
+}
+
+// Adds the S CTAs' sums of this thread's channel for the rank's TN / S tokens and
+// finishes them; `part` is the shared address of the channel's first sum. The
+// reads of eight tokens from all CTAs are in flight together.
+template <int TN, int S>
+__device__ __forceinline__ void join(const Epilogue& e, uint32_t part, int rank, int64_t t0, const float* sx, int n,
+                                     float sw, float b) {
+    constexpr int PER = TN / S, R = PER < 8 ? PER : 8;
+    uint32_t from[S];
+#pragma unroll
+    for (int p = 0; p < S; ++p) from[p] = map_to(part, p);
+#pragma unroll 1
+    for (int i = 0; i < PER; i += R) {
+        const int c = rank * PER + i;
+        if (t0 + c >= e.T) break;
+        int v[S][R];
+#pragma unroll
+        for (int p = 0; p < S; ++p)
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[p][j]) : "r"(from[p] + (c + j) * BM * 4));
+        float scale = sx[0];
+#pragma unroll
+        for (int k = 1; k < (TN + 31) / 32; ++k) scale = c / 32 == k ? sx[k] : scale;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            int sum = 0;
+#pragma unroll
+            for (int p = 0; p < S; ++p) sum += v[p][j];
+            const float f = (float)sum * __shfl_sync(~0u, scale, (c + j) % 32) * sw;
+            if (t0 + c + j < e.T && n < e.N) store_out(e, t0 + c + j, n, e.bias ? f + b : f);
+        }
+    }
+}
+
+template <int TN, bool TMA>
+__global__ void __launch_bounds__(panel_threads(TMA), 1)
+panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, Rows8 w,
+             Rows8 x, int K, int S, int ttiles, Epilogue e) {
+    using P = Panel<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t bars[2 * P::STAGES + 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort;
+    const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * P::STAGES, done = empty0 + 8 * P::STAGES;
+    const uint32_t base = smem_u32(smem);
+    const int rank = (int)(blockIdx.x % (unsigned)S);
+    const unsigned tile = blockIdx.x / (unsigned)S;
+    const int64_t t0 = (int64_t)(tile % (unsigned)ttiles) * TN;
+    const int m0 = (int)(tile / (unsigned)ttiles) * BM;
+    const int nkb = (K + BK - 1) / BK;                     // K blocks; this CTA's: kb0 .. kb0 + nk - 1
+    const int kb0 = (int)((int64_t)nkb * rank / S), nk = (int)((int64_t)nkb * (rank + 1) / S) - kb0;
+
+    auto load = [&](int it, int s) {                       // block kb0 + it into stage s (one thread)
+        const uint32_t fb = full0 + 8 * s, dst = base + s * P::STAGE;
+        mbar_expect(fb, P::STAGE);
+        const int k = (kb0 + it) * BK;
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+            :: "r"(dst), "l"((uint64_t)&map_w), "r"(k), "r"(m0), "r"(fb) : "memory");
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+            :: "r"(dst + BM * BK), "l"((uint64_t)&map_x), "r"(k), "r"((int)t0), "r"(fb) : "memory");
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < P::STAGES; ++i) {
+            mbar_init(full0 + 8 * i, TMA ? 1 : LOADERS);
+            mbar_init(empty0 + 8 * i, 1);
+        }
+        mbar_init(done, 1);
+        abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (TMA)                                           // the ring is filled before anything else is set up
+            for (int it = 0; it < min(nk, P::STAGES); ++it) load(it, it);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&tmem_slot)), "r"(P::COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (TMA && elect_one()) {
+            int it = min(nk, P::STAGES);
+            Ring<P::STAGES> r;
+            for (; it < nk; ++it, r.next()) {
+                if (!mbar_wait(empty0 + 8 * r.s, r.phase, &abort)) break;
+                load(it, r.s);
+            }
+            if (abort)                                     // copies in flight land before the CTA ends
+                for (int j = max(it - P::STAGES, 0); j < it; ++j)
+                    mbar_wait(full0 + 8 * (j % P::STAGES), (j / P::STAGES) & 1, nullptr);
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint64_t d0 = sw128_desc(base);
+            int left = K - kb0 * BK;
+            Ring<P::STAGES> r;
+            for (int it = 0; it < nk; ++it, r.next(), left -= BK) {
+                if (!mbar_wait(full0 + 8 * r.s, r.phase, &abort)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t d = d0 + (uint64_t)(r.s * (P::STAGE >> 4));
+                mma_block<1>(tmem, d, d + (BM * BK >> 4), idesc_i8(BM, TN), left, it > 0);
+                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                             :: "r"(empty0 + 8 * r.s) : "memory");
+            }
+            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                         :: "r"(done) : "memory");
+        }
+    } else if (!TMA) {                                     // the other warps fill the stages
+        const int lw = warp - 2;
+        for (int it = 0; it < nk; ++it) {
+            const int s = it % P::STAGES;
+            if (it >= P::STAGES && !__all_sync(~0u, mbar_wait(empty0 + 8 * s, (it / P::STAGES - 1) & 1, &abort))) break;
+            const uint32_t dst = base + s * P::STAGE;
+            const int k = (kb0 + it) * BK;
+            constexpr int LW = LOADERS / 32, R = 8, RX = TN / LW < R ? TN / LW : R;
+#pragma unroll 1
+            for (int r = lw; r < BM; r += LW * R) load_rows<R>(w, m0, r, LW, k, K, dst, lane);
+#pragma unroll 1
+            for (int r = lw; r < TN; r += LW * RX) load_rows<RX>(x, t0, r, LW, k, K, dst + BM * BK, lane);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(full0 + 8 * s) : "memory");
+        }
+    }
+
+    const int q4 = warp & 3, row = q4 * 32 + lane, n = m0 + row;
+    const bool epi = warp >= 2 && warp < 6;
+    const float sw = epi && n < e.N ? e.sw[n] : 0.0f, b = epi && n < e.N && e.bias ? e.bias[n] : 0.0f;
+    constexpr int NSX = (TN + 31) / 32;
+    float sx[NSX];
+    if (epi) get_scales<NSX>(e, t0, sx);
+    bool ok = true;
+    __syncwarp();
+    if (epi) {
+        ok = warp_wait(done, 0, nullptr);
+        ok = __all_sync(~0u, ok && !abort);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16);
+    if (S == 1) {
+        if (epi && ok) {
+#pragma unroll
+            for (int c = 0; c < TN; c += 16) {
+                int r[16];
+                tmem_ld16(r, lanes + c);
+                put16(e, r, t0 + c, sx[c / 32], c % 32, n, sw, b);
+            }
+        }
+    } else {
+        int* part = reinterpret_cast<int*>(smem);          // [TN][128]: every MMA has read its stage
+        if (epi && ok) {
+#pragma unroll
+            for (int c = 0; c < TN; c += 16) {
+                int r[16];
+                tmem_ld16(r, lanes + c);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) part[(c + j) * BM + row] = r[j];
+            }
+        }
+        cluster_sync();
+        if (epi && ok) {
+            if (S == 2) join<TN, 2>(e, base + row * 4, rank, t0, sx, n, sw, b);
+            else if (S == 4) join<TN, 4>(e, base + row * 4, rank, t0, sx, n, sw, b);
+            else join<TN, 8>(e, base + row * 4, rank, t0, sx, n, sw, b);
+        }
+        cluster_sync();                                    // no CTA leaves while its sums are read
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(P::COLS));
+}
+
+// ---- pairs: many tokens --------------------------------------------------------
+//
+// Two CTAs on neighbouring SMs share each MMA (cta_group::2): 256 tokens (rows)
+// by TN channels (columns), each CTA loading its 128 tokens and half of the
+// channels, so that an SM takes in 32 KB for 128 x 256 x 128 products where it
+// would alone take in 48 KB. Persistent: the pair's two accumulators alternate,
+// and a tile's epilogue runs under the next tile's products.
+constexpr int PAIR_EPI_WARPS = 8;
+constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
+constexpr int RASTER = 8;                                  // tiles of tokens walked together
+constexpr int ROW_BYTES = 64;                              // of a token's outputs staged at a time
+
+template <int TN>
+struct Pair {
+    static constexpr int STAGE = (BM + TN / 2) * BK;
+    static constexpr int STAGES = TN == 256 ? 6 : 8;
+    static constexpr int FACTORS = 2 * (TN / 2) * 4;       // a warp's channel scales and biases
+    static constexpr int STAGED = 32 * ROW_BYTES;          // a warp's outputs on their way out
+    static constexpr int SMEM = STAGES * STAGE + PAIR_EPI_WARPS * (FACTORS + STAGED) + 1024;
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A warp's 32 tokens (from t; lane = token, scale sx) by `cols` channels (from n),
+// 64 bytes of outputs a token at a time: staged in shared memory (16-byte piece
+// p of row r at p ^ (r / 2 % 4): no bank conflicts either way) and written out
+// with four lanes a row where rows begin on 16-byte boundaries, else a row's
+// values side by side.
+template <class O>
+__device__ __forceinline__ void put_rows(const Epilogue& e, uint32_t taddr, int64_t t, int n, int cols, float sx,
+                                         const float* factors, uint8_t* staged, int lane) {
+    constexpr int CH = ROW_BYTES / (int)sizeof(O);
+    const int rows = (int)min((int64_t)32, e.T - t);
+    O* const out = static_cast<O*>(e.out) + t * e.ldo + n;
+#pragma unroll 1
+    for (int c = 0; c < cols && n + c < e.N; c += CH) {
+        int r[CH];
+        if (CH == 32) tmem_ld32(r, taddr + c);
+        else tmem_ld16(r, taddr + c);
+        uint32_t v[16];
+#pragma unroll
+        for (int j = 0; j < CH; j += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(factors + c + j);
+            const float4 b = *reinterpret_cast<const float4*>(factors + cols + c + j);
+            const float v0 = (float)r[j] * sx * w.x + b.x, v1 = (float)r[j + 1] * sx * w.y + b.y,
+                        v2 = (float)r[j + 2] * sx * w.z + b.z, v3 = (float)r[j + 3] * sx * w.w + b.w;
+            if constexpr (sizeof(O) == 4) {
+                v[j] = __float_as_uint(v0); v[j + 1] = __float_as_uint(v1);
+                v[j + 2] = __float_as_uint(v2); v[j + 3] = __float_as_uint(v3);
+            } else {
+                v[j / 2] = pack2(v0, v1, O());
+                v[j / 2 + 1] = pack2(v2, v3, O());
+            }
+        }
+        __syncwarp();                                      // the last piece has been read
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            *reinterpret_cast<uint4*>(staged + lane * ROW_BYTES + 16 * (p ^ (lane / 2 % 4))) =
+                make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+        __syncwarp();
+        if (e.vec && n + c + CH <= e.N) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 8 * i + lane / 4, p = lane % 4;
+                const uint4 o = *reinterpret_cast<const uint4*>(staged + row * ROW_BYTES + 16 * (p ^ (row / 2 % 4)));
+                if (row < rows) *reinterpret_cast<uint4*>(out + row * e.ldo + c + p * (16 / (int)sizeof(O))) = o;
+            }
+        } else {
+            for (int row = lane / CH; row < rows; row += 32 / CH) {
+                const int col = lane % CH, at = col * (int)sizeof(O);
+                if (n + c + col < e.N)
+                    out[row * e.ldo + c + col] = *reinterpret_cast<const O*>(
+                        staged + row * ROW_BYTES + 16 * (at / 16 ^ (row / 2 % 4)) + at % 16);
+            }
+        }
+    }
+}
+
+template <int TN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, int K, int mt,
+            int nt, Epilogue e) {
+    using P = Pair<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t bars[2 * P::STAGES + 5];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort;
+    const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * P::STAGES, tfull0 = empty0 + 8 * P::STAGES,
+                   tempty0 = tfull0 + 16, drain = tempty0 + 16;
+    const uint32_t base = smem_u32(smem);
+    const int rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+    const int nk = (K + BK - 1) / BK;
+    const int64_t tiles = (int64_t)mt * nt;
+
+    if (tid == 0) {
+        for (int i = 0; i < P::STAGES; ++i) {
+            mbar_init(full0 + 8 * i, 1);                   // used in the first CTA only
+            mbar_init(empty0 + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(tfull0 + 8 * i, 1);
+            mbar_init(tempty0 + 8 * i, 2 * PAIR_EPI_WARPS);   // used in the first CTA only
+        }
+        mbar_init(drain, 1);
+        abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&tmem_slot)), "r"((uint32_t)(2 * TN)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+
+    auto tile_at = [&](int64_t i, int64_t& t0, int& n0) {  // the first token and channel of tile i
+        const int64_t group = i / ((int64_t)RASTER * nt), r = i - group * RASTER * nt;
+        const int wide = min(RASTER, mt - (int)group * RASTER);
+        t0 = (group * RASTER + r % wide) * 2 * BM;
+        n0 = (int)(r / wide) * TN;
+    };
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const uint32_t lead0 = map_to(full0, 0);       // the first CTA's barriers
+            Ring<P::STAGES> r;
+            uint32_t first = 1;                            // the ring's first round waits for nothing
+            bool ok = true;
+            for (int64_t i = pair; ok && i < tiles; i += npairs) {
+                int n0;
+                int64_t t0;
+                tile_at(i, t0, n0);
+                const int y0 = (int)t0 + rank * BM, y1 = n0 + rank * (TN / 2);
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!first && !mbar_wait(empty0 + 8 * r.s, r.phase ^ 1u, &abort)) { ok = false; break; }
+                    if (rank == 0) mbar_expect(full0 + 8 * r.s, 2 * P::STAGE);
+                    const uint32_t fb = lead0 + 8 * r.s, dst = base + r.s * P::STAGE;
+                    asm volatile(
+                        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+                        " [%0], [%1, {%2, %3}], [%4];"
+                        :: "r"(dst), "l"((uint64_t)&map_x), "r"(kb * BK), "r"(y0), "r"(fb) : "memory");
+                    asm volatile(
+                        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+                        " [%0], [%1, {%2, %3}], [%4];"
+                        :: "r"(dst + BM * BK), "l"((uint64_t)&map_w), "r"(kb * BK), "r"(y1), "r"(fb) : "memory");
+                    r.next();
+                    if (r.s == 0) first = 0;
+                }
+            }
+            if (!ok) {                                     // copies in flight land before the CTA ends: the
+                const long long c0 = clock64();            // second CTA cannot wait on the first's barriers
+                while (clock64() - c0 < (1ll << 24)) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            const uint64_t d0 = sw128_desc(base);
+            Ring<P::STAGES> r;
+            Ring<2> acc;
+            bool ok = true;
+            for (int64_t i = pair; ok && i < tiles; i += npairs, acc.next()) {
+                if (i >= pair + 2 * (int64_t)npairs && !mbar_wait(tempty0 + 8 * acc.s, acc.phase ^ 1u, &abort)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                int left = K;
+                for (int kb = 0; kb < nk; ++kb, r.next(), left -= BK) {
+                    if (!mbar_wait(full0 + 8 * r.s, r.phase, &abort)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t d = d0 + (uint64_t)(r.s * (P::STAGE >> 4));
+                    mma_block<2>(tmem + acc.s * TN, d, d + (BM * BK >> 4), idesc_i8(2 * BM, TN), left, kb > 0);
+                    asm volatile(
+                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                        :: "r"(empty0 + 8 * r.s), "h"((uint16_t)3) : "memory");
+                }
+                if (!ok) break;
+                asm volatile(
+                    "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                    :: "r"(tfull0 + 8 * acc.s), "h"((uint16_t)3) : "memory");
+            }
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(drain) : "memory");
+            mbar_wait(drain, 0, nullptr);                  // every MMA issued has completed
+        }
+    } else {
+        const int q4 = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter, column half
+        constexpr int COLS = TN / 2;
+        uint8_t* mine = smem + P::STAGES * P::STAGE + (warp - 2) * (P::FACTORS + P::STAGED);
+        float* factors = reinterpret_cast<float*>(mine);
+        uint8_t* staged = mine + P::FACTORS;
+        Ring<2> acc;
+        for (int64_t i = pair; i < tiles; i += npairs, acc.next()) {
+            int n0;
+            int64_t t0;
+            tile_at(i, t0, n0);
+            const int64_t t = t0 + rank * BM + q4 * 32;
+            const int n = n0 + half * COLS;
+            const float sx = t + lane < e.T ? e.sx[t + lane] : 0.0f;
+            __syncwarp();
+            for (int c = lane; c < COLS; c += 32) {
+                factors[c] = n + c < e.N ? e.sw[n + c] : 0.0f;
+                factors[COLS + c] = e.bias && n + c < e.N ? e.bias[n + c] : 0.0f;
+            }
+            __syncwarp();
+            if (!warp_wait(tfull0 + 8 * acc.s, acc.phase, &abort)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t taddr = tmem + ((uint32_t)(q4 * 32) << 16) + acc.s * TN + half * COLS;
+            if (t < e.T) {
+                if (e.type == JHQ_BF16) put_rows<__nv_bfloat16>(e, taddr, t, n, COLS, sx, factors, staged, lane);
+                else if (e.type == JHQ_F16) put_rows<__half>(e, taddr, t, n, COLS, sx, factors, staged, lane);
+                else put_rows<float>(e, taddr, t, n, COLS, sx, factors, staged, lane);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                             :: "r"(map_to(tempty0 + 8 * acc.s, 0)) : "memory");
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();                                        // no MMA or arrival still heads for the other CTA
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t)(2 * TN)));
+}
+
+// ---- host ------------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult qr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
+            qr == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+    });
+    if (!fn) fail(JHQ_EDEVICE, "q8_matmul: cuTensorMapEncodeTiled unavailable");
+    return fn;
+}
+
+// What a tensor map takes: rows that begin on 16-byte boundaries.
+bool on_boundaries(const jhq_q8_rows* r) {
+    return (uintptr_t)r->q % 16 == 0 && (r->rows == 1 || (r->ld % 16 == 0 && r->ld < (1ll << 40)));
+}
+
+// Boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside the array.
+CUtensorMap make_map(const jhq_q8_rows* r, int box_rows) {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {(cuuint64_t)r->dim, (cuuint64_t)r->rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(r->rows == 1 ? (r->dim + 15) / 16 * 16 : r->ld)};
+    const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult rc = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r->q, dims, strides, box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) fail(JHQ_EDEVICE, "q8_matmul: tensor map encoding failed");
+    return m;
+}
+
+constexpr int SMS = 148;
+
+template <int TN, bool TMA>
+void launch_panels(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    once_per_device(done, [] {
+        JHQ_CUDA(cudaFuncSetAttribute(panel_kernel<TN, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Panel<TN>::SMEM));
+    });
+    const int64_t ttiles = ceil_div(x->rows, TN), tiles = ttiles * ceil_div(w->rows, BM);
+    const int nkb = (int)ceil_div(x->dim, BK);
+    int S = 1;                     
+    while (S < 8 && tiles * S * 2 <= SMS && nkb >= 4 * S) S *= 2;
+    if (tiles * S > INT32_MAX) fail(JHQ_EINVAL, "q8_matmul: too many rows");
+    CUtensorMap mw{}, mx{};
+    if (TMA) { mw = make_map(w, BM); mx = make_map(x, TN); }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * S));
+    cfg.blockDim = dim3(panel_threads(TMA));
+    cfg.dynamicSmemBytes = Panel<TN>::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)S;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    JHQ_CUDA(cudaLaunchKernelEx(&cfg, panel_kernel<TN, TMA>, mw, mx, Rows8{w->q, w->ld, w->rows},
+                                Rows8{x->q, x->ld, x->rows}, (int)x->dim, S, (int)ttiles, e));
+}
+
+template <bool TMA>
+void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaStream_t s) {
+    if (x->rows <= 16) launch_panels<16, TMA>(x, w, e, s);
+    else if (x->rows <= 32) launch_panels<32, TMA>(x, w, e, s);
+    else if (x->rows <= 64) launch_panels<64, TMA>(x, w, e, s);
+    else launch_panels<128, TMA>(x, w, e, s);
+}
+
+// Microseconds of the busiest pair with tiles of 256 tokens by tn channels, from what a K block and a tile cost when
+// measured alone: 0.20 and 2.0 with 128 channels, 0.275 and 3.3 with 256. The narrow tile wins where the wide one leaves
+// pairs idle (512 x 1024 x 1024: 7.3 against 9.4 us), the wide one elsewhere (32768 x 8192 x 8192: 1293 against 1862 us).
+double pair_cost(const jhq_q8_rows* x, const jhq_q8_rows* w, int tn, double block, double tile) {
+    const int64_t tiles = ceil_div(x->rows, 2 * BM) * ceil_div(w->rows, tn);
+    return (double)ceil_div(tiles, SMS / 2) * ((double)ceil_div(x->dim, BK) * block + tile);
+}
+
+template <int TN>
+void pairs(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    once_per_device(done, [] {
+        JHQ_CUDA(cudaFuncSetAttribute(pair_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Pair<TN>::SMEM));
+    });
+    const int64_t mt = ceil_div(x->rows, 2 * BM), nt = ceil_div(w->rows, TN);
+    const unsigned grid = 2 * (unsigned)std::min<int64_t>(SMS / 2, mt * nt);
+    pair_kernel<TN><<<grid, PAIR_THREADS, Pair<TN>::SMEM, s>>>(make_map(x, BM), make_map(w, TN / 2), (int)x->dim,
+                                                               (int)mt, (int)nt, e);
 }
 
 }  // namespace
@@ -92,9 +800,12 @@ void q8_matmul(const jhq_q8_rows* x, const jhq_q8_rows* w, const jhq_view* bias,
             fail(JHQ_EINVAL, "q8_matmul: bias must be 1 x w's rows of float32");
     }
     const Epilogue e{x->scale, w->scale, bias ? (const float*)bias->data : nullptr, out->data, out->ld,
-                     x->rows, (int)w->rows, out->type};
-    const dim3 grid((unsigned)ceil_div(x->rows, TILE), (unsigned)ceil_div(w->rows, TILE));
-    simple_kernel<<<grid, 256, 0, s>>>(x->q, x->ld, w->q, w->ld, (int)x->dim, e);
+                     x->rows, (int)w->rows, out->type,
+                     (uintptr_t)out->data % 16 == 0 && out->ld % (out->type == JHQ_F32 ? 4 : 8) == 0};
+    if (!on_boundaries(x) || !on_boundaries(w)) panels<false>(x, w, e, s);
+    else if (x->rows <= 128) panels<true>(x, w, e, s);
+    else if (pair_cost(x, w, 128, 0.20, 2.0) < pair_cost(x, w, 256, 0.275, 3.3)) pairs<128>(x, w, e, s);
+    else pairs<256>(x, w, e, s);
     JHQ_LAUNCH_CHECK();
     count_launch();
 }
