@@ -651,31 +651,50 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         float* factors = reinterpret_cast<float*>(mine);
         uint8_t* staged = mine + P::FACTORS;
         Ring<2> acc;
-        for (int64_t i = pair; i < tiles; i += npairs, acc.next()) {
+        float sx = 0.0f, sw[COLS / 32], b[COLS / 32];      // of the next tile: this lane's token, every 32nd channel
+        int64_t t = 0;
+        int n = 0;
+        auto fetch = [&](int64_t i) {
+            if (i >= tiles) return;
             int n0;
-            int64_t t0;
-            tile_at(i, t0, n0);
-            const int64_t t = t0 + rank * BM + q4 * 32;
-            const int n = n0 + half * COLS;
-            const float sx = t + lane < e.T ? e.sx[t + lane] : 0.0f;
+            tile_at(i, t, n0);
+            t += rank * BM + q4 * 32;
+            n = n0 + half * COLS;
+            sx = t + lane < e.T ? e.sx[t + lane] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < COLS / 32; ++c) {
+                const int at = n + 32 * c + lane;
+                sw[c] = at < e.N ? e.sw[at] : 0.0f;
+                b[c] = e.bias && at < e.N ? e.bias[at] : 0.0f;
+            }
+        };
+        fetch(pair);
+        for (int64_t i = pair; i < tiles; i += npairs, acc.next()) {
+            const int64_t t1 = t;
+            const int n1 = n;
+            const float sx1 = sx;
             __syncwarp();
-            for (int c = lane; c < COLS; c += 32) {
-                factors[c] = n + c < e.N ? e.sw[n + c] : 0.0f;
-                factors[COLS + c] = e.bias && n + c < e.N ? e.bias[n + c] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < COLS / 32; ++c) {
+                factors[32 * c + lane] = sw[c];
+                factors[COLS + 32 * c + lane] = b[c];
             }
             __syncwarp();
+            fetch(i + npairs);                             // arrives under this tile's products and outputs
             if (!warp_wait(tfull0 + 8 * acc.s, acc.phase, &abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem + ((uint32_t)(q4 * 32) << 16) + acc.s * TN + half * COLS;
-            if (t < e.T) {
-                if (e.type == JHQ_BF16) put_rows<__nv_bfloat16>(e, taddr, t, n, COLS, sx, factors, staged, lane);
-                else if (e.type == JHQ_F16) put_rows<__half>(e, taddr, t, n, COLS, sx, factors, staged, lane);
-                else put_rows<float>(e, taddr, t, n, COLS, sx, factors, staged, lane);
+            if (t1 < e.T) {
+                if (e.type == JHQ_BF16) put_rows<__nv_bfloat16>(e, taddr, t1, n1, COLS, sx1, factors, staged, lane);
+                else if (e.type == JHQ_F16) put_rows<__half>(e, taddr, t1, n1, COLS, sx1, factors, staged, lane);
+                else put_rows<float>(e, taddr, t1, n1, COLS, sx1, factors, staged, lane);
             }
+            // relaxed: the arrival hands over TMEM alone, whose reads have completed;
+            // a release would wait for the outputs' stores as well
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0)
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];"
                              :: "r"(map_to(tempty0 + 8 * acc.s, 0)) : "memory");
         }
     }
