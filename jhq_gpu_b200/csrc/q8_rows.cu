@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -17,13 +18,15 @@
 
 namespace jhq {
 
+static constexpr int64_t MAX_ROW = 1ll << 30;             // values: indexes within a row are 32-bit
+
 void q8_check_view(const jhq_view* v, const char* what) {
     const std::string w(what);
     if (!v) fail(JHQ_EINVAL, w + ": null");
     if (v->type != JHQ_F32 && v->type != JHQ_F16 && v->type != JHQ_BF16)
         fail(JHQ_EINVAL, w + ": unknown type");
-    if (v->rows < 0 || v->cols < 1 || v->cols > INT32_MAX)
-        fail(JHQ_EINVAL, w + ": rows must be >= 0 and cols in 1..2^31-1");
+    if (v->rows < 0 || v->cols < 1 || v->cols > MAX_ROW)
+        fail(JHQ_EINVAL, w + ": rows must be >= 0 and cols in 1..2^30");
     if (v->rows > 1 && v->ld < v->cols) fail(JHQ_EINVAL, w + ": ld is smaller than a row");
     if (v->rows > 0 && !v->data) fail(JHQ_EINVAL, w + ": null data");
     if ((uintptr_t)v->data % (v->type == JHQ_F32 ? 4 : 2))
@@ -33,8 +36,8 @@ void q8_check_view(const jhq_view* v, const char* what) {
 void q8_check_rows(const jhq_q8_rows* r, const char* what) {
     const std::string w(what);
     if (!r) fail(JHQ_EINVAL, w + ": null");
-    if (r->rows < 0 || r->dim < 1 || r->dim > INT32_MAX)
-        fail(JHQ_EINVAL, w + ": rows must be >= 0 and dim in 1..2^31-1");
+    if (r->rows < 0 || r->dim < 1 || r->dim > MAX_ROW)
+        fail(JHQ_EINVAL, w + ": rows must be >= 0 and dim in 1..2^30");
     if (r->groups < 1 || r->dim % r->groups) fail(JHQ_EINVAL, w + ": groups must divide dim");
     if (r->rows > 1 && r->ld < r->dim) fail(JHQ_EINVAL, w + ": ld is smaller than a row");
     if (r->rows > 0 && (!r->q || !r->scale)) fail(JHQ_EINVAL, w + ": null buffer");
@@ -43,139 +46,370 @@ void q8_check_rows(const jhq_q8_rows* r, const char* what) {
 
 namespace {
 
-constexpr int THREADS = 256;
 constexpr uint32_t INF_BITS = 0x7f800000u;
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void store(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_float(float* p, float v) { *p = v; }
+__device__ __forceinline__ void from_float(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Block-wide sum and maximum, returned to every thread.
-__device__ float2 block_sum_max(float sum, uint32_t top, float* red) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    top = __reduce_max_sync(~0u, top);
-    __syncthreads();                                     // red is free again
-    if (lane == 0) { red[2 * warp] = sum; red[2 * warp + 1] = __uint_as_float(top); }
-    __syncthreads();
-    sum = 0.0f;
-    top = 0;
-    for (int i = 0; i < THREADS / 32; ++i) {
-        sum += red[2 * i];
-        top = max(top, __float_as_uint(red[2 * i + 1]));
+// V values from p as floats, in accesses of up to 16 bytes; zeros behind the
+// first `left`. p is aligned to the accesses where V > 1.
+template <int V, class T>
+__device__ __forceinline__ void load(const T* p, int left, float* out) {
+    constexpr int B = V * (int)sizeof(T);
+    if (V > 1 && left >= V) {
+        __align__(16) T v[V];
+        if constexpr (B >= 16) {
+#pragma unroll
+            for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else if constexpr (B == 8) {
+            *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = i < left ? to_float(p[i]) : 0.0f;
+    }
+}
+template <int V, class T>
+__device__ __forceinline__ void put(T* p, int left, const float* in) {
+    constexpr int B = V * (int)sizeof(T);
+    if (V > 1 && left >= V) {
+        __align__(16) T v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) from_float(&v[i], in[i]);
+        if constexpr (B >= 16) {
+#pragma unroll
+            for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+        } else if constexpr (B == 8) {
+            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) from_float(p + i, in[i]);
+    }
+}
+
+// rint(g * (127 * (1 / a))) as a byte. A tiny a would make 1 / a infinite: both
+// are scaled by 2^64 first (exact). Adding 1.5 * 2^23 rounds to the nearest whole
+// number, ties to even, and leaves it in the low byte.
+struct Quant {
+    float pre, inv;
+    bool fine;                                           // a is positive and finite; else the bytes are 0
+    __device__ explicit Quant(float a) {
+        pre = a < 1e-30f ? 0x1p64f : 1.0f;
+        fine = a > 0.0f && __float_as_uint(a) < INF_BITS;
+        inv = fine ? 127.0f * (1.0f / (a * pre)) : 0.0f;
+    }
+    __device__ uint32_t operator()(float g) const {
+        return fine ? __float_as_uint(g * pre * inv + 12582912.0f) & 255u : 0u;
+    }
+};
+template <int V>
+__device__ __forceinline__ void put_bytes(int8_t* p, int left, const uint32_t* v) {
+    if (V > 1 && left >= V) {
+        uint32_t w[(V + 3) / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            w[i] = __byte_perm(__byte_perm(v[4 * i], v[4 * i + 1], 0x0040), __byte_perm(v[4 * i + 2], v[4 * i + 3], 0x0040), 0x5410);
+        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        else if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = (int8_t)v[i];
+    }
+}
+
+// Sum and maximum over a team of TPR threads: lanes of a warp, or a whole block.
+template <int TPR>
+__device__ __forceinline__ float2 team_sum_max(float sum, uint32_t top, float2* red) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) {
+        sum += __shfl_xor_sync(~0u, sum, o);
+        top = max(top, __shfl_xor_sync(~0u, top, o));
+    }
+    if (TPR > 32) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (lane == 0) red[warp] = make_float2(sum, __uint_as_float(top));
+        __syncthreads();
+        const float2 v = lane < TPR / 32 ? red[lane] : make_float2(0.0f, 0.0f);
+        sum = v.x;
+        top = __float_as_uint(v.y);
+#pragma unroll
+        for (int o = TPR / 64; o; o >>= 1) {
+            sum += __shfl_xor_sync(~0u, sum, o);
+            top = max(top, __shfl_xor_sync(~0u, top, o));
+        }
+        sum = __shfl_sync(~0u, sum, 0);
+        top = __shfl_sync(~0u, top, 0);
     }
     return make_float2(sum, __uint_as_float(top));
 }
 
-// q = rint(g * (127 * (1 / a))). A tiny a would make 1 / a infinite: both are
-// scaled by 2^64 first (exact).
-struct Quant {
-    float pre, inv;
-    __device__ explicit Quant(float a) {
-        pre = a < 1e-30f ? 0x1p64f : 1.0f;
-        inv = a > 0.0f && __float_as_uint(a) < INF_BITS ? 127.0f * (1.0f / (a * pre)) : 0.0f;
-    }
-    __device__ int8_t operator()(float g) const {
-        return inv == 0.0f ? (int8_t)0 : (int8_t)__float2int_rn(g * pre * inv);
-    }
+struct Args {
+    const void* x;
+    int64_t ldx;
+    const void *res, *weight;                            // null: none, ones
+    void* res_out;                                       // null: not wanted; may be res
+    int64_t ldr, ldo;
+    int w32;                                             // weight is float32, else x's type
+    float eps;
+    int8_t* q;
+    int64_t ldq;
+    float* scale;
+    const int64_t* slots;
+    int64_t nslots;
+    unsigned teams;                                      // rows times groups
+    int groups, d;                                       // d: values of a group
 };
 
-template <class T, class R>
-__global__ void __launch_bounds__(THREADS)
-rms_norm_kernel(const T* __restrict__ x, int64_t ldx, const R* res, int64_t ldr,
-                const void* __restrict__ weight, int w32, float eps, R* res_out, int64_t ldo,
-                int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale, int d) {
-    __shared__ float red[2 * THREADS / 32];
-    const int64_t row = blockIdx.x;
-    x += row * ldx;
-    if (res) res += row * ldr;
-    if (res_out) res_out += row * ldo;
-    q += row * ldq;
-    auto h_of = [&](int j) {
-        const float v = to_float(x[j]);
-        return res ? v + to_float(res[j]) : v;
+constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+// Blocks of one SM that the registers are held down for: 1024 to 1536 threads.
+constexpr int blocks_of(int tpr) { return tpr < 512 ? 5 : tpr == 512 ? 2 : 1; }
+
+// One pass over a row (a group, when the cache is written): a team of TPR threads
+// holds EPT values each in registers, in 16-byte pieces (VEC) or single values, so
+// x and the residual are read once and every output is written once. Bound by those
+// bytes; rows as short as 16 values share a warp, longer ones get a warp or a block, so that
+// a single row is spread over as many loads as it has and many rows keep all SMs' loads in flight.
+template <class T, class R, int TPR, int EPT, bool VEC, bool NORM>
+__global__ void __launch_bounds__(block_of(TPR), blocks_of(TPR))
+rows_kernel(const __grid_constant__ Args a) {
+    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = EPT / V;
+    __shared__ float2 red[3][32];
+    const unsigned team = TPR > block_of(TPR) / 2 ? blockIdx.x : blockIdx.x * (block_of(TPR) / TPR) + threadIdx.x / TPR;
+    const int me = threadIdx.x % TPR;
+    const bool in = team < a.teams;
+    const int64_t row = a.groups == 1 ? team : team / (unsigned)a.groups;
+    const int g = a.groups == 1 ? 0 : (int)(team - (unsigned)row * (unsigned)a.groups);
+    const int64_t to = !in ? -1 : a.slots ? a.slots[row] : row;
+    const bool wanted = to >= 0 && (NORM || to < a.nslots);
+    const int d = wanted ? a.d : 0;
+    const T* x = static_cast<const T*>(a.x) + (in ? row * a.ldx + (int64_t)g * a.d : 0);
+    auto at = [&](int i) { return (i * TPR + me) * V; };   // the thread's i-th piece
+
+    float h[EPT];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load<V>(x + at(i), d - at(i), h + i * V);
+    if (NORM && a.res) {
+        const R* res = static_cast<const R*>(a.res) + (in ? row * a.ldr : 0);
+        float r[EPT];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load<V>(res + at(i), d - at(i), r + i * V);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) h[i] += r[i];
+    }
+    auto weigh = [&](float* w, int i) {                  // the weights of piece i
+        if (!NORM || !a.weight) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = 1.0f;
+        } else if (a.w32) load<V>(static_cast<const float*>(a.weight) + at(i), d - at(i), w);
+        else load<V>(static_cast<const T*>(a.weight) + at(i), d - at(i), w);
     };
-    auto w_of = [&](int j) {
-        if (!weight) return 1.0f;
-        return w32 ? static_cast<const float*>(weight)[j] : to_float(static_cast<const T*>(weight)[j]);
-    };
+    if (NORM && a.res_out) {
+        R* o = static_cast<R*>(a.res_out) + (in ? row * a.ldo : 0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) put<V>(o + at(i), d - at(i), h + i * V);
+    }
     float sum = 0.0f;
     uint32_t top = 0;                                    // bits of |g| order like |g|, NaN on top
-    for (int j = threadIdx.x; j < d; j += THREADS) {
-        const float h = h_of(j);
-        sum += h * h;
-        top = max(top, __float_as_uint(fabsf(h * w_of(j))));
-    }
-    const float2 st = block_sum_max(sum, top, red);
-    float a = st.y, sc = 1.0f, step = a / (127.0f * sqrtf(st.x / (float)d + eps));
-    if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && a >= 0x1p-100f && a <= 0x1p120f)) {
-        // near the ends of float32's range: again with h scaled by a power of two
-        uint32_t hm = 0;
-        for (int j = threadIdx.x; j < d; j += THREADS) hm = max(hm, __float_as_uint(fabsf(h_of(j))));
-        const float htop = block_sum_max(0.0f, hm, red).y;
-        if (htop > 0.0f && __float_as_uint(htop) < INF_BITS) {
-            const int e = min(max(ilogbf(htop), -126), 126);
-            sc = ldexpf(1.0f, -e);
-            sum = 0.0f;
-            top = 0;
-            for (int j = threadIdx.x; j < d; j += THREADS) {
-                const float h = h_of(j) * sc;
-                sum += h * h;
-                top = max(top, __float_as_uint(fabsf(h * w_of(j))));
+    auto gather = [&](float by) {
+        sum = 0.0f;
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float w[V];
+            weigh(w, i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = h[i * V + j] * by;
+                if (NORM) sum += v * v;
+                top = max(top, __float_as_uint(v * w[j]) & 0x7fffffffu);
             }
-            const float2 s2 = block_sum_max(sum, top, red);
-            a = s2.y;
-            step = (float)((double)a / (127.0 * sqrt((double)s2.x / d + (double)eps * sc * sc)));
+        }
+    };
+    gather(1.0f);
+    const float2 st = team_sum_max<TPR>(sum, top, red[0]);
+    float top_g = st.y, by = 1.0f, step;
+    if (NORM) {
+        step = top_g / (127.0f * sqrtf(st.x / (float)a.d + a.eps));
+        if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
+            // near the ends of float32's range: again with h scaled by a power of two
+            uint32_t hm = 0;
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) hm = max(hm, __float_as_uint(fabsf(h[i])));
+            const float htop = team_sum_max<TPR>(0.0f, hm, red[1]).y;
+            if (htop > 0.0f && __float_as_uint(htop) < INF_BITS) {
+                by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
+                gather(by);
+                const float2 s2 = team_sum_max<TPR>(sum, top, red[2]);
+                top_g = s2.y;
+                step = (float)((double)top_g / (127.0 * sqrt((double)s2.x / a.d + (double)a.eps * by * by)));
+            }
+        }
+    } else {
+        step = top_g / 127.0f;
+    }
+    const Quant quant(top_g);
+    int8_t* q = a.q + (wanted ? to * a.ldq + (int64_t)g * a.d : 0);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float w[V];
+        weigh(w, i);
+        uint32_t b[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) b[j] = quant(NORM ? h[i * V + j] * by * w[j] : h[i * V + j]);
+        put_bytes<V>(q + at(i), d - at(i), b);
+    }
+    if (me == 0 && wanted)
+        a.scale[to * a.groups + g] = !(__float_as_uint(top_g) < INF_BITS) ? __uint_as_float(0x7fffffffu)
+                                     : top_g > 0.0f                       ? step
+                                                                          : 0.0f;
+}
+
+// Rows longer than a block's registers: the row is read twice (thrice near the
+// ends of float32's range).
+constexpr int LONG_THREADS = 1024;
+template <class T, class R, bool NORM>
+__global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_constant__ Args a) {
+    __shared__ float2 red[3][32];
+    const int64_t row = a.groups == 1 ? blockIdx.x : blockIdx.x / (unsigned)a.groups;
+    const int g = a.groups == 1 ? 0 : (int)(blockIdx.x % (unsigned)a.groups);
+    const int64_t to = a.slots ? a.slots[row] : row;
+    if (to < 0 || (!NORM && to >= a.nslots)) return;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx + (int64_t)g * a.d;
+    const R* res = a.res ? static_cast<const R*>(a.res) + row * a.ldr : nullptr;
+    R* res_out = a.res_out ? static_cast<R*>(a.res_out) + row * a.ldo : nullptr;
+    int8_t* q = a.q + to * a.ldq + (int64_t)g * a.d;
+    auto h_of = [&](int j) {
+        const float v = to_float(x[j]);
+        return NORM && res ? v + to_float(res[j]) : v;
+    };
+    auto w_of = [&](int j) {
+        if (!NORM || !a.weight) return 1.0f;
+        return a.w32 ? static_cast<const float*>(a.weight)[j] : to_float(static_cast<const T*>(a.weight)[j]);
+    };
+    auto gather = [&](float by, float2* r) {
+        float sum = 0.0f;
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) {
+            const float h = h_of(j) * by;
+            if (NORM) sum += h * h;
+            top = max(top, __float_as_uint(h * w_of(j)) & 0x7fffffffu);
+        }
+        return team_sum_max<LONG_THREADS>(sum, top, r);
+    };
+    const float2 st = gather(1.0f, red[0]);
+    float top_g = st.y, by = 1.0f, step = top_g / 127.0f;
+    if (NORM) {
+        step = top_g / (127.0f * sqrtf(st.x / (float)a.d + a.eps));
+        if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
+            uint32_t hm = 0;
+            for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max(hm, __float_as_uint(fabsf(h_of(j))));
+            const float htop = team_sum_max<LONG_THREADS>(0.0f, hm, red[1]).y;
+            if (htop > 0.0f && __float_as_uint(htop) < INF_BITS) {
+                by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
+                const float2 s2 = gather(by, red[2]);
+                top_g = s2.y;
+                step = (float)((double)top_g / (127.0 * sqrt((double)s2.x / a.d + (double)a.eps * by * by)));
+            }
         }
     }
-    const Quant quant(a);
-    for (int j = threadIdx.x; j < d; j += THREADS) {
-        const float h = h_of(j);
-        if (res_out) store(res_out + j, h);
-        q[j] = quant(h * sc * w_of(j));
+    const Quant quant(top_g);
+#pragma unroll 4
+    for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) {
+        const float h = h_of(j), w = w_of(j);
+        if (NORM && res_out) from_float(res_out + j, h);
+        q[j] = (int8_t)quant(h * by * w);
     }
-    if (threadIdx.x == 0) {
-        const bool fine = __float_as_uint(a) < INF_BITS;
-        scale[row] = !fine ? __uint_as_float(0x7fffffffu) : a > 0.0f ? step : 0.0f;
-    }
-}
-
-template <class T>
-__global__ void __launch_bounds__(THREADS)
-write_kernel(const T* __restrict__ x, int64_t ldx, const int64_t* __restrict__ slots,
-             int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale, int64_t nslots, int groups,
-             int gdim) {
-    __shared__ float red[2 * THREADS / 32];
-    const int64_t row = blockIdx.x / groups;
-    const int g = (int)(blockIdx.x % groups);
-    const int64_t slot = slots ? slots[row] : row;
-    if (slot < 0 || slot >= nslots) return;
-    x += row * ldx + (int64_t)g * gdim;
-    q += slot * ldq + (int64_t)g * gdim;
-    uint32_t top = 0;
-    for (int j = threadIdx.x; j < gdim; j += THREADS)
-        top = max(top, __float_as_uint(fabsf(to_float(x[j]))));
-    const float a = block_sum_max(0.0f, top, red).y;
-    const Quant quant(a);
-    for (int j = threadIdx.x; j < gdim; j += THREADS) q[j] = quant(to_float(x[j]));
     if (threadIdx.x == 0)
-        scale[slot * groups + g] =
-            __float_as_uint(a) < INF_BITS ? a / 127.0f : __uint_as_float(0x7fffffffu);
+        a.scale[to * a.groups + g] = !(__float_as_uint(top_g) < INF_BITS) ? __uint_as_float(0x7fffffffu)
+                                     : top_g > 0.0f                       ? step
+                                                                          : 0.0f;
 }
 
-template <class T>
-__global__ void __launch_bounds__(THREADS)
+template <class T, class R, int TPR, int EPT, bool VEC, bool NORM>
+void launch_team(const Args& a, cudaStream_t s) {
+    constexpr unsigned per = block_of(TPR) / TPR;
+    rows_kernel<T, R, TPR, EPT, VEC, NORM><<<(a.teams + per - 1) / per, block_of(TPR), 0, s>>>(a);
+}
+// The smallest team whose registers hold a row.
+template <class T, class R, bool VEC, bool NORM>
+void launch_rows(const Args& a, cudaStream_t s) {
+    const int d = a.d;
+    if (!NORM && d <= 32) launch_team<T, R, 4, 8, VEC, NORM>(a, s);
+    else if (!NORM && d <= 128) launch_team<T, R, 16, 8, VEC, NORM>(a, s);
+    else if (d <= 256) launch_team<T, R, 32, 8, VEC, NORM>(a, s);
+    else if (d <= 512) launch_team<T, R, 32, 16, VEC, NORM>(a, s);
+    else if (d <= 4096) launch_team<T, R, 256, 16, VEC, NORM>(a, s);
+    else if (d <= 8192) launch_team<T, R, 512, 16, VEC, NORM>(a, s);
+    else if (d <= 16384) launch_team<T, R, 1024, 16, VEC, NORM>(a, s);
+    else long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
+}
+
+bool on_bytes(const void* p, int64_t ld, int size, int rows_of, int64_t rows) {
+    return (uintptr_t)p % rows_of == 0 && (rows <= 1 || ld * size % rows_of == 0);
+}
+
+// Reads rows back: V values of a row a thread (32 bytes of output where rows
+// allow it), TPR threads a row. Bound by the bytes: one in, sizeof(T) out a value.
+template <class T, int V>
+struct alignas(V * sizeof(T)) Piece {
+    T v[V];
+};
+template <class T, int V>
+__global__ void __launch_bounds__(256)
 read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
-            const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int groups, int gdim) {
-    const int64_t row = blockIdx.x;
+            const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
+            int gdim, int dim) {
+    const int64_t row = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+    if (row >= rows) return;
     const int64_t slot = slots ? slots[row] : row;
     const bool there = slot >= 0 && slot < nslots;
+    q += there ? slot * ldq : 0;
+    scale += there ? slot * groups : 0;
     out += row * ldo;
-    for (int j = threadIdx.x; j < groups * gdim; j += THREADS)
-        store(out + j, there ? scale[slot * groups + j / gdim] * (float)q[slot * ldq + j] : 0.0f);
+    for (int j = (blockIdx.y * tpr + threadIdx.x % tpr) * V; j < dim; j += (int)gridDim.y * tpr * V) {
+        Piece<int8_t, V> b;
+        float sc = 0.0f;
+        if (there) {
+            b = *reinterpret_cast<const Piece<int8_t, V>*>(q + j);
+            sc = scale[groups == 1 ? 0 : (unsigned)j / (unsigned)gdim];
+        }
+        alignas(32) T v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) from_float(&v[i], there ? sc * (float)b.v[i] : 0.0f);
+        if constexpr (V * sizeof(T) == 32) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                         :: "l"(out + j), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                            "r"(w[7]) : "memory");
+        } else {
+            *reinterpret_cast<Piece<T, V>*>(out + j) = *reinterpret_cast<const Piece<T, V>*>(v);
+        }
+    }
+}
+
+template <class T, int V>
+bool try_read(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, cudaStream_t s) {
+    const int gdim = (int)(c->dim / c->groups), dim = (int)c->dim;
+    if (V > 1 && (gdim % V || !on_bytes(c->q, c->ld, 1, V, c->rows) ||
+                  !on_bytes(out->data, out->ld, sizeof(T), V * (int)sizeof(T), out->rows)))
+        return false;
+    const int tpr = std::min(256, next_pow2((int)ceil_div(dim, V)));
+    const int64_t blocks = ceil_div(out->rows, 256 / tpr);
+    if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(65535, ceil_div(dim, tpr * V)));
+    read_kernel<T, V><<<grid, 256, 0, s>>>(c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows,
+                                           tpr, c->groups, gdim, dim);
+    return true;
 }
 
 template <class F>
@@ -217,15 +451,30 @@ void q8_rms_norm(const jhq_view* x, const jhq_view* residual, const jhq_view* we
         fail(JHQ_EINVAL, "q8_rms_norm: residual and residual_out must have one type");
     if (x->rows == 0) return;
     if (x->rows > INT32_MAX) fail(JHQ_EINVAL, "q8_rms_norm: too many rows");
+    Args a{};
+    a.x = x->data;
+    a.ldx = x->ld;
+    if (residual) { a.res = residual->data; a.ldr = residual->ld; }
+    if (residual_out) { a.res_out = residual_out->data; a.ldo = residual_out->ld; }
+    if (weight) { a.weight = weight->data; a.w32 = weight->type == JHQ_F32; }
+    a.eps = eps;
+    a.q = out->q;
+    a.ldq = out->ld;
+    a.scale = out->scale;
+    a.teams = (unsigned)x->rows;
+    a.groups = 1;
+    a.d = (int)x->cols;
     by_type(x->type, [&](auto t) {
         using T = decltype(t);
+        constexpr int V = 16 / (int)sizeof(T);
         auto go = [&](auto r) {
             using R = decltype(r);
-            rms_norm_kernel<T, R><<<(unsigned)x->rows, THREADS, 0, s>>>(
-                (const T*)x->data, x->ld, residual ? (const R*)residual->data : nullptr,
-                residual ? residual->ld : 0, weight ? weight->data : nullptr,
-                weight && weight->type == JHQ_F32, eps, residual_out ? (R*)residual_out->data : nullptr,
-                residual_out ? residual_out->ld : 0, out->q, out->ld, out->scale, (int)x->cols);
+            const int rb = std::min(16, V * (int)sizeof(R));
+            const bool vec = on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) && on_bytes(a.q, a.ldq, 1, V, x->rows) &&
+                             on_bytes(a.res, a.ldr, sizeof(R), rb, x->rows) &&
+                             on_bytes(a.res_out, a.ldo, sizeof(R), rb, x->rows) && (uintptr_t)a.weight % 16 == 0;
+            if (vec) launch_rows<T, R, true, true>(a, s);
+            else launch_rows<T, R, false, true>(a, s);
         };
         if (rtype == x->type) go(t);
         else go(float());
@@ -241,12 +490,25 @@ void q8_write(const jhq_view* x, const int64_t* slots, const jhq_q8_rows* cache,
     if (!slots && x->rows > cache->rows) fail(JHQ_EINVAL, "q8_write: more rows than the cache has");
     if ((uintptr_t)slots % 8) fail(JHQ_EINVAL, "q8_write: slots are not aligned to 8 bytes");
     if (x->rows == 0 || cache->rows == 0) return;
-    if (x->rows * cache->groups > INT32_MAX) fail(JHQ_EINVAL, "q8_write: too many rows");
+    if (x->rows > INT32_MAX / cache->groups) fail(JHQ_EINVAL, "q8_write: too many rows");
+    Args a{};
+    a.x = x->data;
+    a.ldx = x->ld;
+    a.q = cache->q;
+    a.ldq = cache->ld;
+    a.scale = cache->scale;
+    a.slots = slots;
+    a.nslots = cache->rows;
+    a.teams = (unsigned)(x->rows * cache->groups);
+    a.groups = cache->groups;
+    a.d = (int)(cache->dim / cache->groups);
     by_type(x->type, [&](auto t) {
         using T = decltype(t);
-        write_kernel<T><<<(unsigned)(x->rows * cache->groups), THREADS, 0, s>>>(
-            (const T*)x->data, x->ld, slots, cache->q, cache->ld, cache->scale, cache->rows,
-            cache->groups, (int)(cache->dim / cache->groups));
+        constexpr int V = 16 / (int)sizeof(T);
+        const bool vec = (a.groups == 1 || a.d % V == 0) && on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) &&
+                         on_bytes(a.q, a.ldq, 1, V, cache->rows);
+        if (vec) launch_rows<T, T, true, false>(a, s);
+        else launch_rows<T, T, false, false>(a, s);
     });
     JHQ_LAUNCH_CHECK();
     count_launch();
@@ -259,12 +521,10 @@ void q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out
     if (!slots && out->rows > cache->rows) fail(JHQ_EINVAL, "q8_read: more rows than the cache has");
     if ((uintptr_t)slots % 8) fail(JHQ_EINVAL, "q8_read: slots are not aligned to 8 bytes");
     if (out->rows == 0) return;
-    if (out->rows > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
     by_type(out->type, [&](auto t) {
         using T = decltype(t);
-        read_kernel<T><<<(unsigned)out->rows, THREADS, 0, s>>>(
-            cache->q, cache->ld, cache->scale, cache->rows, slots, (T*)out->data, out->ld,
-            cache->groups, (int)(cache->dim / cache->groups));
+        if (!try_read<T, 32 / (int)sizeof(T)>(cache, slots, out, s) && !try_read<T, 4>(cache, slots, out, s))
+            try_read<T, 1>(cache, slots, out, s);
     });
     JHQ_LAUNCH_CHECK();
     count_launch();
