@@ -55,102 +55,129 @@ __device__ __forceinline__ void from_float(float* p, float v) { *p = v; }
 __device__ __forceinline__ void from_float(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// V values from p as floats, in accesses of up to 16 bytes; zeros behind the
-// first `left`. p is aligned to the accesses where V > 1.
-template <int V, class T>
+// How a thread touches its piece of V values at p, of which the first `left` are
+// the row's: single values (V = 1), whole pieces of 16 bytes of x (all or nothing
+// is the row's), or whole pieces with a ragged last one, value by value.
+enum Access { SINGLE, WHOLE, RAGGED };
+
+__device__ __forceinline__ uint4 load16(const void* p) {     // not kept in L1, which is left to the weights
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+// STREAM: read once, past L1.
+template <Access A, int V, bool STREAM, class T>
 __device__ __forceinline__ void load(const T* p, int left, float* out) {
     constexpr int B = V * (int)sizeof(T);
-    if (V > 1 && left >= V) {
-        __align__(16) T v[V];
-        if constexpr (B >= 16) {
-#pragma unroll
-            for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
-        } else if constexpr (B == 8) {
-            *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
-    } else {
+    if (A == RAGGED && left > 0 && left < V) {
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = i < left ? to_float(p[i]) : 0.0f;
+        return;
     }
-}
-template <int V, class T>
-__device__ __forceinline__ void put(T* p, int left, const float* in) {
-    constexpr int B = V * (int)sizeof(T);
-    if (V > 1 && left >= V) {
-        __align__(16) T v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) from_float(&v[i], in[i]);
+    alignas(16) T v[V];
+    if (left > 0) {
         if constexpr (B >= 16) {
 #pragma unroll
-            for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+            for (int i = 0; i < B / 16; ++i)
+                reinterpret_cast<uint4*>(v)[i] = STREAM ? load16(reinterpret_cast<const uint4*>(p) + i) : reinterpret_cast<const uint4*>(p)[i];
         } else if constexpr (B == 8) {
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+            *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p);
+        } else {
+            v[0] = p[0];
         }
     } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) from_float(&v[i], 0.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
+}
+template <Access A, int V, class T>
+__device__ __forceinline__ void put(T* p, int left, const float* in) {
+    constexpr int B = V * (int)sizeof(T);
+    if (A == RAGGED && left < V) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < left) from_float(p + i, in[i]);
+        return;
+    }
+    if (left <= 0) return;
+    alignas(16) T v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) from_float(&v[i], in[i]);
+    if constexpr (B >= 16) {
+#pragma unroll
+        for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+    } else if constexpr (B == 8) {
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+    } else {
+        p[0] = v[0];
     }
 }
-
-// rint(g * (127 * (1 / a))) as a byte. A tiny a would make 1 / a infinite: both
-// are scaled by 2^64 first (exact). Adding 1.5 * 2^23 rounds to the nearest whole
-// number, ties to even, and leaves it in the low byte.
-struct Quant {
-    float pre, inv;
-    bool fine;                                           // a is positive and finite; else the bytes are 0
-    __device__ explicit Quant(float a) {
-        pre = a < 1e-30f ? 0x1p64f : 1.0f;
-        fine = a > 0.0f && __float_as_uint(a) < INF_BITS;
-        inv = fine ? 127.0f * (1.0f / (a * pre)) : 0.0f;
-    }
-    __device__ uint32_t operator()(float g) const {
-        return fine ? __float_as_uint(g * pre * inv + 12582912.0f) & 255u : 0u;
-    }
-};
-template <int V>
+template <Access A, int V>
 __device__ __forceinline__ void put_bytes(int8_t* p, int left, const uint32_t* v) {
-    if (V > 1 && left >= V) {
-        uint32_t w[(V + 3) / 4];
+    if (A == RAGGED && left < V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = (int8_t)v[i];
+        return;
+    }
+    if (left <= 0) return;
+    if constexpr (V == 1) {
+        p[0] = (int8_t)v[0];
+    } else {
+        uint32_t w[V / 4];
 #pragma unroll
         for (int i = 0; i < V / 4; ++i)
             w[i] = __byte_perm(__byte_perm(v[4 * i], v[4 * i + 1], 0x0040), __byte_perm(v[4 * i + 2], v[4 * i + 3], 0x0040), 0x5410);
         if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-        else if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) p[i] = (int8_t)v[i];
+        else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     }
 }
 
+// rint(g * (127 * (1 / a))) in the low byte of the result: adding 1.5 * 2^23
+// rounds to the nearest whole number, ties to even. A tiny a would make 1 / a
+// infinite: both are scaled by 2^64 first (exact).
+struct Quant {
+    float pre, inv;
+    bool fine;                                           // a is positive and finite; else all bytes are 0
+    __device__ explicit Quant(float a) {
+        pre = a < 1e-30f ? 0x1p64f : 1.0f;
+        fine = a > 0.0f && __float_as_uint(a) < INF_BITS;
+        inv = fine ? 127.0f * __frcp_rn(a * pre) : 0.0f;
+    }
+    __device__ uint32_t plain(float g) const { return __float_as_uint(g * inv + 12582912.0f); }   // fine, pre = 1
+    __device__ uint32_t operator()(float g) const { return fine ? plain(g * pre) : 0u; }
+};
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // Sum and maximum over a team of TPR threads: lanes of a warp, or a whole block.
 template <int TPR>
-__device__ __forceinline__ float2 team_sum_max(float sum, uint32_t top, float2* red) {
+__device__ __forceinline__ float2 team_sum_max(float sum, float top, float2* red) {
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) {
         sum += __shfl_xor_sync(~0u, sum, o);
-        top = max(top, __shfl_xor_sync(~0u, top, o));
+        top = max_nan(top, __shfl_xor_sync(~0u, top, o));
     }
     if (TPR > 32) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        if (lane == 0) red[warp] = make_float2(sum, __uint_as_float(top));
+        if (lane == 0) red[warp] = make_float2(sum, top);
         __syncthreads();
-        const float2 v = lane < TPR / 32 ? red[lane] : make_float2(0.0f, 0.0f);
+        const float2 v = red[lane % (TPR > 32 ? TPR / 32 : 1)];
         sum = v.x;
-        top = __float_as_uint(v.y);
+        top = v.y;
 #pragma unroll
         for (int o = TPR / 64; o; o >>= 1) {
             sum += __shfl_xor_sync(~0u, sum, o);
-            top = max(top, __shfl_xor_sync(~0u, top, o));
+            top = max_nan(top, __shfl_xor_sync(~0u, top, o));
         }
-        sum = __shfl_sync(~0u, sum, 0);
-        top = __shfl_sync(~0u, top, 0);
     }
-    return make_float2(sum, __uint_as_float(top));
+    return make_float2(sum, top);
 }
+__device__ __forceinline__ bool is_finite(float a) { return (__float_as_uint(a) & 0x7fffffffu) < INF_BITS; }
 
 struct Args {
     const void* x;
@@ -169,59 +196,59 @@ struct Args {
     int groups, d;                                       // d: values of a group
 };
 
-constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
-// Blocks of one SM that the registers are held down for: 1024 to 1536 threads.
-constexpr int blocks_of(int tpr) { return tpr < 512 ? 5 : tpr == 512 ? 2 : 1; }
+constexpr int SMS = 148;
+constexpr int block_of(int tpr) { return tpr < 64 ? 128 : tpr; }
+// Blocks an SM holds: 1024 threads with up to 16 values each, 768 with 32.
+constexpr int blocks_of(int tpr, int ept) { return (ept == 32 ? 768 : 1024) / block_of(tpr) > 0 ? (ept == 32 ? 768 : 1024) / block_of(tpr) : 1; }
 
 // One pass over a row (a group, when the cache is written): a team of TPR threads
-// holds EPT values each in registers, in 16-byte pieces (VEC) or single values, so
-// x and the residual are read once and every output is written once. Bound by those
-// bytes; rows as short as 16 values share a warp, longer ones get a warp or a block, so that
-// a single row is spread over as many loads as it has and many rows keep all SMs' loads in flight.
-template <class T, class R, int TPR, int EPT, bool VEC, bool NORM>
-__global__ void __launch_bounds__(block_of(TPR), blocks_of(TPR))
+// holds EPT values each in registers, so x and the residual are read once and
+// every output is written once. Bound by those bytes, as long as a thread has
+// enough values that the instructions spent on a row and not on a value (addresses,
+// the team's reductions, the reciprocal) stay few. Short groups share a warp, rows
+// to 1024 values have a warp, longer ones a block.
+template <class T, class R, int TPR, int EPT, Access A, bool NORM>
+__global__ void __launch_bounds__(block_of(TPR), blocks_of(TPR, EPT))
 rows_kernel(const __grid_constant__ Args a) {
-    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = EPT / V;
+    constexpr int V = A == SINGLE ? 1 : 16 / (int)sizeof(T), NV = EPT / V;
+    constexpr unsigned PER = block_of(TPR) / TPR;          // teams a block
     __shared__ float2 red[3][32];
-    const unsigned team = TPR > block_of(TPR) / 2 ? blockIdx.x : blockIdx.x * (block_of(TPR) / TPR) + threadIdx.x / TPR;
     const int me = threadIdx.x % TPR;
-    const bool in = team < a.teams;
-    const int64_t row = a.groups == 1 ? team : team / (unsigned)a.groups;
-    const int g = a.groups == 1 ? 0 : (int)(team - (unsigned)row * (unsigned)a.groups);
-    const int64_t to = !in ? -1 : a.slots ? a.slots[row] : row;
-    const bool wanted = to >= 0 && (NORM || to < a.nslots);
-    const int d = wanted ? a.d : 0;
-    const T* x = static_cast<const T*>(a.x) + (in ? row * a.ldx + (int64_t)g * a.d : 0);
+    const unsigned team = blockIdx.x * PER + (PER > 1 ? threadIdx.x / TPR : 0);
+    const bool in = team < a.teams;                        // else the team only keeps the warp's shuffles company
+    const int64_t row = !in ? 0 : a.groups == 1 ? team : team / (unsigned)a.groups;
+    const int64_t off = !in ? 0 : (int64_t)(team - (unsigned)row * (unsigned)a.groups) * a.d;   // of the group
+    const int64_t slot = !in ? -1 : a.slots ? a.slots[row] : row;
+    const int d = in ? a.d : 0;
     auto at = [&](int i) { return (i * TPR + me) * V; };   // the thread's i-th piece
 
     float h[EPT];
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx + off;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load<V>(x + at(i), d - at(i), h + i * V);
+    for (int i = 0; i < NV; ++i) load<A, V, true>(x + at(i), d - at(i), h + i * V);
     if (NORM && a.res) {
-        const R* res = static_cast<const R*>(a.res) + (in ? row * a.ldr : 0);
+        const R* res = static_cast<const R*>(a.res) + row * a.ldr;
         float r[EPT];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) load<V>(res + at(i), d - at(i), r + i * V);
+        for (int i = 0; i < NV; ++i) load<A, V, true>(res + at(i), d - at(i), r + i * V);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) h[i] += r[i];
     }
-    auto weigh = [&](float* w, int i) {                  // the weights of piece i
+    if (NORM && a.res_out) {
+        R* o = static_cast<R*>(a.res_out) + row * a.ldo;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) put<A, V>(o + at(i), d - at(i), h + i * V);
+    }
+    auto weigh = [&](float* w, int i) {                    // the weights of piece i
         if (!NORM || !a.weight) {
 #pragma unroll
             for (int j = 0; j < V; ++j) w[j] = 1.0f;
-        } else if (a.w32) load<V>(static_cast<const float*>(a.weight) + at(i), d - at(i), w);
-        else load<V>(static_cast<const T*>(a.weight) + at(i), d - at(i), w);
+        } else if (a.w32) load<A, V, false>(static_cast<const float*>(a.weight) + at(i), a.d - at(i), w);
+        else load<A, V, false>(static_cast<const T*>(a.weight) + at(i), a.d - at(i), w);
     };
-    if (NORM && a.res_out) {
-        R* o = static_cast<R*>(a.res_out) + (in ? row * a.ldo : 0);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) put<V>(o + at(i), d - at(i), h + i * V);
-    }
-    float sum = 0.0f;
-    uint32_t top = 0;                                    // bits of |g| order like |g|, NaN on top
+    float sum = 0.0f, top = 0.0f;
     auto gather = [&](float by) {
-        sum = 0.0f;
-        top = 0;
+        sum = top = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float w[V];
@@ -229,48 +256,60 @@ rows_kernel(const __grid_constant__ Args a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float v = h[i * V + j] * by;
-                if (NORM) sum += v * v;
-                top = max(top, __float_as_uint(v * w[j]) & 0x7fffffffu);
+                if (NORM) sum = __fmaf_rn(v, v, sum);
+                top = max_nan(top, fabsf(v * w[j]));
             }
         }
     };
     gather(1.0f);
     const float2 st = team_sum_max<TPR>(sum, top, red[0]);
-    float top_g = st.y, by = 1.0f, step;
-    if (NORM) {
-        step = top_g / (127.0f * sqrtf(st.x / (float)a.d + a.eps));
-        if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
-            // near the ends of float32's range: again with h scaled by a power of two
-            uint32_t hm = 0;
+    float top_g = st.y, by = 1.0f;
+    double sum_sq = st.x;
+    if (NORM && !(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
+        // near the ends of float32's range: again with h scaled by a power of two
+        float hm = 0.0f;
 #pragma unroll
-            for (int i = 0; i < EPT; ++i) hm = max(hm, __float_as_uint(fabsf(h[i])));
-            const float htop = team_sum_max<TPR>(0.0f, hm, red[1]).y;
-            if (htop > 0.0f && __float_as_uint(htop) < INF_BITS) {
-                by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
-                gather(by);
-                const float2 s2 = team_sum_max<TPR>(sum, top, red[2]);
-                top_g = s2.y;
-                step = (float)((double)top_g / (127.0 * sqrt((double)s2.x / a.d + (double)a.eps * by * by)));
-            }
+        for (int i = 0; i < EPT; ++i) hm = max_nan(hm, fabsf(h[i]));
+        const float htop = team_sum_max<TPR>(0.0f, hm, red[1]).y;
+        if (htop > 0.0f && is_finite(htop)) {
+            by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
+            gather(by);
+            const float2 s2 = team_sum_max<TPR>(sum, top, red[2]);
+            top_g = s2.y;
+            sum_sq = s2.x;
         }
-    } else {
-        step = top_g / 127.0f;
     }
     const Quant quant(top_g);
-    int8_t* q = a.q + (wanted ? to * a.ldq + (int64_t)g * a.d : 0);
+    const bool wanted = in && slot >= 0 && (NORM || slot < a.nslots);
+    int8_t* q = a.q + (wanted ? slot * a.ldq + off : 0);
+    const int keep = wanted ? d : 0;
+    if (quant.fine && quant.pre == 1.0f && by == 1.0f) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float w[V];
-        weigh(w, i);
-        uint32_t b[V];
+        for (int i = 0; i < NV; ++i) {
+            float w[V];
+            weigh(w, i);
+            uint32_t b[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) b[j] = quant(NORM ? h[i * V + j] * by * w[j] : h[i * V + j]);
-        put_bytes<V>(q + at(i), d - at(i), b);
+            for (int j = 0; j < V; ++j) b[j] = quant.plain(NORM ? h[i * V + j] * w[j] : h[i * V + j]);
+            put_bytes<A, V>(q + at(i), keep - at(i), b);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float w[V];
+            weigh(w, i);
+            uint32_t b[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[j] = quant(NORM ? h[i * V + j] * by * w[j] : h[i * V + j]);
+            put_bytes<A, V>(q + at(i), keep - at(i), b);
+        }
     }
-    if (me == 0 && wanted)
-        a.scale[to * a.groups + g] = !(__float_as_uint(top_g) < INF_BITS) ? __uint_as_float(0x7fffffffu)
-                                     : top_g > 0.0f                       ? step
-                                                                          : 0.0f;
+    if (me == 0 && wanted) {
+        float step = top_g / 127.0f;
+        if (NORM) step = by == 1.0f ? top_g / (127.0f * sqrtf((float)sum_sq / (float)a.d + a.eps))
+                                    : (float)((double)top_g / (127.0 * sqrt(sum_sq / a.d + (double)a.eps * by * by)));
+        a.scale[slot * a.groups + (int)(off / a.d)] = !is_finite(top_g) ? __uint_as_float(0x7fffffffu) : top_g > 0.0f ? step : 0.0f;
+    }
 }
 
 // Rows longer than a block's registers: the row is read twice (thrice near the
@@ -296,13 +335,12 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
         return a.w32 ? static_cast<const float*>(a.weight)[j] : to_float(static_cast<const T*>(a.weight)[j]);
     };
     auto gather = [&](float by, float2* r) {
-        float sum = 0.0f;
-        uint32_t top = 0;
+        float sum = 0.0f, top = 0.0f;
 #pragma unroll 4
         for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) {
             const float h = h_of(j) * by;
-            if (NORM) sum += h * h;
-            top = max(top, __float_as_uint(h * w_of(j)) & 0x7fffffffu);
+            if (NORM) sum = __fmaf_rn(h, h, sum);
+            top = max_nan(top, fabsf(h * w_of(j)));
         }
         return team_sum_max<LONG_THREADS>(sum, top, r);
     };
@@ -311,10 +349,10 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
     if (NORM) {
         step = top_g / (127.0f * sqrtf(st.x / (float)a.d + a.eps));
         if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
-            uint32_t hm = 0;
-            for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max(hm, __float_as_uint(fabsf(h_of(j))));
+            float hm = 0.0f;
+            for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max_nan(hm, fabsf(h_of(j)));
             const float htop = team_sum_max<LONG_THREADS>(0.0f, hm, red[1]).y;
-            if (htop > 0.0f && __float_as_uint(htop) < INF_BITS) {
+            if (htop > 0.0f && is_finite(htop)) {
                 by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
                 const float2 s2 = gather(by, red[2]);
                 top_g = s2.y;
@@ -330,27 +368,28 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
         q[j] = (int8_t)quant(h * by * w);
     }
     if (threadIdx.x == 0)
-        a.scale[to * a.groups + g] = !(__float_as_uint(top_g) < INF_BITS) ? __uint_as_float(0x7fffffffu)
-                                     : top_g > 0.0f                       ? step
-                                                                          : 0.0f;
+        a.scale[to * a.groups + g] = !is_finite(top_g) ? __uint_as_float(0x7fffffffu) : top_g > 0.0f ? step : 0.0f;
 }
 
-template <class T, class R, int TPR, int EPT, bool VEC, bool NORM>
+template <class T, class R, int TPR, int EPT, Access A, bool NORM>
 void launch_team(const Args& a, cudaStream_t s) {
     constexpr unsigned per = block_of(TPR) / TPR;
-    rows_kernel<T, R, TPR, EPT, VEC, NORM><<<(a.teams + per - 1) / per, block_of(TPR), 0, s>>>(a);
+    rows_kernel<T, R, TPR, EPT, A, NORM><<<(a.teams - 1) / per + 1, block_of(TPR), 0, s>>>(a);
 }
 // The smallest team whose registers hold a row.
-template <class T, class R, bool VEC, bool NORM>
+template <class T, class R, Access A, bool NORM>
 void launch_rows(const Args& a, cudaStream_t s) {
     const int d = a.d;
-    if (!NORM && d <= 32) launch_team<T, R, 4, 8, VEC, NORM>(a, s);
-    else if (!NORM && d <= 128) launch_team<T, R, 16, 8, VEC, NORM>(a, s);
-    else if (d <= 256) launch_team<T, R, 32, 8, VEC, NORM>(a, s);
-    else if (d <= 512) launch_team<T, R, 32, 16, VEC, NORM>(a, s);
-    else if (d <= 4096) launch_team<T, R, 256, 16, VEC, NORM>(a, s);
-    else if (d <= 8192) launch_team<T, R, 512, 16, VEC, NORM>(a, s);
-    else if (d <= 16384) launch_team<T, R, 1024, 16, VEC, NORM>(a, s);
+    if (!NORM && d <= 32) launch_team<T, R, 4, 8, A, NORM>(a, s);
+    else if (!NORM && d <= 64) launch_team<T, R, 4, 16, A, NORM>(a, s);
+    else if (!NORM && d <= 128) launch_team<T, R, 8, 16, A, NORM>(a, s);
+    else if (d <= 256) launch_team<T, R, NORM ? 32 : 16, NORM ? 8 : 16, A, NORM>(a, s);
+    else if (d <= 512) launch_team<T, R, 32, 16, A, NORM>(a, s);
+    else if (d <= 1024) launch_team<T, R, 32, 32, A, NORM>(a, s);
+    else if (d <= 2048) launch_team<T, R, 64, 32, A, NORM>(a, s);
+    else if (d <= 4096) launch_team<T, R, 128, 32, A, NORM>(a, s);
+    else if (d <= 8192) launch_team<T, R, 256, 32, A, NORM>(a, s);
+    else if (d <= 16384) launch_team<T, R, 512, 32, A, NORM>(a, s);
     else long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
 }
 
@@ -364,35 +403,62 @@ template <class T, int V>
 struct alignas(V * sizeof(T)) Piece {
     T v[V];
 };
-template <class T, int V>
-__global__ void __launch_bounds__(256)
+// Value i of a piece as a float: the byte + 128 as the low bits of 2^23, less
+// 2^23 + 128 (exact); half the cost of a conversion.
+template <int V>
+__device__ __forceinline__ float byte_float(const Piece<int8_t, V>& b, int i) {
+    if constexpr (V == 1) return (float)b.v[0];
+    else {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(b.v)[i / 4] ^ 0x80808080u;
+        return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + i % 4)) - 8388736.0f;
+    }
+}
+
+template <class T, int V, int U>
+__global__ void __launch_bounds__(256, U == 1 ? 6 : 4)
 read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
             const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
             int gdim, int dim) {
-    const int64_t row = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
-    if (row >= rows) return;
-    const int64_t slot = slots ? slots[row] : row;
-    const bool there = slot >= 0 && slot < nslots;
-    q += there ? slot * ldq : 0;
-    scale += there ? slot * groups : 0;
-    out += row * ldo;
-    for (int j = (blockIdx.y * tpr + threadIdx.x % tpr) * V; j < dim; j += (int)gridDim.y * tpr * V) {
-        Piece<int8_t, V> b;
-        float sc = 0.0f;
-        if (there) {
-            b = *reinterpret_cast<const Piece<int8_t, V>*>(q + j);
-            sc = scale[groups == 1 ? 0 : (unsigned)j / (unsigned)gdim];
-        }
-        alignas(32) T v[V];
+    const int per = 256 / tpr;
+    const int64_t row0 = (int64_t)blockIdx.x * per * U + threadIdx.x / tpr;
+    const int8_t* from[U];
+    const float* fac[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) from_float(&v[i], there ? sc * (float)b.v[i] : 0.0f);
-        if constexpr (V * sizeof(T) == 32) {
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
-            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                         :: "l"(out + j), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
-                            "r"(w[7]) : "memory");
-        } else {
-            *reinterpret_cast<Piece<T, V>*>(out + j) = *reinterpret_cast<const Piece<T, V>*>(v);
+    for (int u = 0; u < U; ++u) {
+        const int64_t row = row0 + u * per, slot = row >= rows ? -1 : slots ? slots[row] : row;
+        const bool there = slot >= 0 && slot < nslots;
+        from[u] = there ? q + slot * ldq : nullptr;
+        fac[u] = scale + (there ? slot * groups : 0);
+    }
+    for (int j = (blockIdx.y * tpr + threadIdx.x % tpr) * V; j < dim; j += (int)gridDim.y * tpr * V) {
+        Piece<int8_t, V> b[U];
+        float sc[U];
+        const unsigned g = groups == 1 ? 0u : (unsigned)j / (unsigned)gdim;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            sc[u] = 0.0f;
+            b[u] = Piece<int8_t, V>{};
+            if (from[u]) {
+                b[u] = *reinterpret_cast<const Piece<int8_t, V>*>(from[u] + j);
+                sc[u] = fac[u][g];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = row0 + u * per;
+            if (row >= rows) break;
+            T* o = out + row * ldo + j;
+            alignas(32) T v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) from_float(&v[i], sc[u] * byte_float(b[u], i));
+            if constexpr (V * sizeof(T) == 32) {
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                             :: "l"(o), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                                "r"(w[7]) : "memory");
+            } else {
+                *reinterpret_cast<Piece<T, V>*>(o) = *reinterpret_cast<const Piece<T, V>*>(v);
+            }
         }
     }
 }
@@ -404,11 +470,13 @@ bool try_read(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, c
                   !on_bytes(out->data, out->ld, sizeof(T), V * (int)sizeof(T), out->rows)))
         return false;
     const int tpr = std::min(256, next_pow2((int)ceil_div(dim, V)));
-    const int64_t blocks = ceil_div(out->rows, 256 / tpr);
+    // two rows a thread once that leaves every SM eight blocks
+    const int U = out->rows >= (int64_t)2 * 8 * SMS * (256 / tpr) ? 2 : 1;
+    const int64_t blocks = ceil_div(out->rows, 256 / tpr * U);
     if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
-    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(65535, ceil_div(dim, tpr * V)));
-    read_kernel<T, V><<<grid, 256, 0, s>>>(c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows,
-                                           tpr, c->groups, gdim, dim);
+    const dim3 grid((unsigned)blocks, (unsigned)(U == 2 ? 1 : std::min<int64_t>(65535, ceil_div(dim, tpr * V))));
+    (U == 2 ? read_kernel<T, V, 2> : read_kernel<T, V, 1>)<<<grid, 256, 0, s>>>(
+        c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows, tpr, c->groups, gdim, dim);
     return true;
 }
 
@@ -473,8 +541,9 @@ void q8_rms_norm(const jhq_view* x, const jhq_view* residual, const jhq_view* we
             const bool vec = on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) && on_bytes(a.q, a.ldq, 1, V, x->rows) &&
                              on_bytes(a.res, a.ldr, sizeof(R), rb, x->rows) &&
                              on_bytes(a.res_out, a.ldo, sizeof(R), rb, x->rows) && (uintptr_t)a.weight % 16 == 0;
-            if (vec) launch_rows<T, R, true, true>(a, s);
-            else launch_rows<T, R, false, true>(a, s);
+            if (!vec) launch_rows<T, R, SINGLE, true>(a, s);
+            else if (a.d % V == 0) launch_rows<T, R, WHOLE, true>(a, s);
+            else launch_rows<T, R, RAGGED, true>(a, s);
         };
         if (rtype == x->type) go(t);
         else go(float());
@@ -507,8 +576,9 @@ void q8_write(const jhq_view* x, const int64_t* slots, const jhq_q8_rows* cache,
         constexpr int V = 16 / (int)sizeof(T);
         const bool vec = (a.groups == 1 || a.d % V == 0) && on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) &&
                          on_bytes(a.q, a.ldq, 1, V, cache->rows);
-        if (vec) launch_rows<T, T, true, false>(a, s);
-        else launch_rows<T, T, false, false>(a, s);
+        if (!vec) launch_rows<T, T, SINGLE, false>(a, s);
+        else if (a.d % V == 0) launch_rows<T, T, WHOLE, false>(a, s);
+        else launch_rows<T, T, RAGGED, false>(a, s);
     });
     JHQ_LAUNCH_CHECK();
     count_launch();
@@ -523,7 +593,8 @@ void q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out
     if (out->rows == 0) return;
     by_type(out->type, [&](auto t) {
         using T = decltype(t);
-        if (!try_read<T, 32 / (int)sizeof(T)>(cache, slots, out, s) && !try_read<T, 4>(cache, slots, out, s))
+        if (!try_read<T, 32 / (int)sizeof(T)>(cache, slots, out, s) && !try_read<T, 8>(cache, slots, out, s) &&
+            !try_read<T, 4>(cache, slots, out, s))
             try_read<T, 1>(cache, slots, out, s);
     });
     JHQ_LAUNCH_CHECK();
