@@ -65,32 +65,54 @@ __device__ __forceinline__ uint4 load16(const void* p) {     // not kept in L1, 
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
-// STREAM: read once, past L1.
+// Loads under a predicate, zeros without: a branch around each would part a
+// thread's loads from one another. STREAM: read once, past L1.
+template <bool STREAM>
+__device__ __forceinline__ void load_if(bool ok, const uint4* p, uint4& v) {
+    if (STREAM)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                     "@p ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                     "@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok) : "memory");
+}
+__device__ __forceinline__ float load_if(bool ok, const float* p) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(v) : "l"(p), "r"((int)ok) : "memory");
+    return __uint_as_float(v);
+}
+__device__ __forceinline__ uint16_t load_if_16(bool ok, const void* p) {
+    uint16_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}" : "=&h"(v) : "l"(p), "r"((int)ok) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_if(bool ok, const __half* p) { return __half2float(__ushort_as_half(load_if_16(ok, p))); }
+__device__ __forceinline__ float load_if(bool ok, const __nv_bfloat16* p) { return __bfloat162float(__ushort_as_bfloat16(load_if_16(ok, p))); }
+
 template <Access A, int V, bool STREAM, class T>
 __device__ __forceinline__ void load(const T* p, int left, float* out) {
     constexpr int B = V * (int)sizeof(T);
-    if (A == RAGGED && left > 0 && left < V) {
+    if constexpr (A == SINGLE) {
+        out[0] = load_if(left > 0, p);
+    } else {
+        if (A == RAGGED && left > 0 && left < V) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = i < left ? to_float(p[i]) : 0.0f;
-        return;
-    }
-    alignas(16) T v[V];
-    if (left > 0) {
+            for (int i = 0; i < V; ++i) out[i] = i < left ? to_float(p[i]) : 0.0f;
+            return;
+        }
+        alignas(16) T v[V];
         if constexpr (B >= 16) {
 #pragma unroll
-            for (int i = 0; i < B / 16; ++i)
-                reinterpret_cast<uint4*>(v)[i] = STREAM ? load16(reinterpret_cast<const uint4*>(p) + i) : reinterpret_cast<const uint4*>(p)[i];
-        } else if constexpr (B == 8) {
-            *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p);
+            for (int i = 0; i < B / 16; ++i) load_if<STREAM>(left > 0, reinterpret_cast<const uint4*>(p) + i, reinterpret_cast<uint4*>(v)[i]);
         } else {
-            v[0] = p[0];
+            static_assert(B == 8, "four 16-bit weights or residuals of float32 rows");
+            *reinterpret_cast<uint2*>(v) = left > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) from_float(&v[i], 0.0f);
+        for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
 }
 template <Access A, int V, class T>
 __device__ __forceinline__ void put(T* p, int left, const float* in) {
@@ -154,23 +176,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// Sum and maximum over a team of TPR threads: lanes of a warp, or a whole block.
-template <int TPR>
+// Sum and maximum over a team: TEAM lanes of a warp, or the block (TEAM = 0).
+template <int TEAM>
 __device__ __forceinline__ float2 team_sum_max(float sum, float top, float2* red) {
 #pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) {
+    for (int o = (TEAM ? TEAM : 32) / 2; o; o >>= 1) {
         sum += __shfl_xor_sync(~0u, sum, o);
         top = max_nan(top, __shfl_xor_sync(~0u, top, o));
     }
-    if (TPR > 32) {
+    if (TEAM == 0) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         if (lane == 0) red[warp] = make_float2(sum, top);
         __syncthreads();
-        const float2 v = red[lane % (TPR > 32 ? TPR / 32 : 1)];
+        const float2 v = lane < (int)blockDim.x / 32 ? red[lane] : make_float2(0.0f, 0.0f);
         sum = v.x;
         top = v.y;
 #pragma unroll
-        for (int o = TPR / 64; o; o >>= 1) {
+        for (int o = 16; o; o >>= 1) {
             sum += __shfl_xor_sync(~0u, sum, o);
             top = max_nan(top, __shfl_xor_sync(~0u, top, o));
         }
@@ -197,24 +219,20 @@ struct Args {
 };
 
 constexpr int SMS = 148;
-constexpr int block_of(int tpr) { return tpr < 64 ? 128 : tpr; }
-// Blocks an SM holds: 1024 threads with up to 16 values each, 768 with 32.
-constexpr int blocks_of(int tpr, int ept) { return (ept == 32 ? 768 : 1024) / block_of(tpr) > 0 ? (ept == 32 ? 768 : 1024) / block_of(tpr) : 1; }
-
 // One pass over a row (a group, when the cache is written): a team of TPR threads
 // holds EPT values each in registers, so x and the residual are read once and
 // every output is written once. Bound by those bytes, as long as a thread has
 // enough values that the instructions spent on a row and not on a value (addresses,
 // the team's reductions, the reciprocal) stay few. Short groups share a warp, rows
-// to 1024 values have a warp, longer ones a block.
-template <class T, class R, int TPR, int EPT, Access A, bool NORM>
-__global__ void __launch_bounds__(block_of(TPR), blocks_of(TPR, EPT))
-rows_kernel(const __grid_constant__ Args a) {
+// to 1024 values have a warp, longer ones a block (TEAM = 0). Registers are held to
+// what lets an SM hold 768 threads with 32 values each, 1024 with fewer.
+constexpr int SHARED_BLOCK = 128, MOST_THREADS = 512;
+template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
+__global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_constant__ Args a) {
     constexpr int V = A == SINGLE ? 1 : 16 / (int)sizeof(T), NV = EPT / V;
-    constexpr unsigned PER = block_of(TPR) / TPR;          // teams a block
     __shared__ float2 red[3][32];
-    const int me = threadIdx.x % TPR;
-    const unsigned team = blockIdx.x * PER + (PER > 1 ? threadIdx.x / TPR : 0);
+    const int TPR = TEAM ? TEAM : (int)blockDim.x, me = TEAM ? threadIdx.x % TEAM : threadIdx.x;
+    const unsigned team = TEAM ? blockIdx.x * (SHARED_BLOCK / (TEAM ? TEAM : 1)) + threadIdx.x / (TEAM ? TEAM : 1) : blockIdx.x;
     const bool in = team < a.teams;                        // else the team only keeps the warp's shuffles company
     const int64_t row = !in ? 0 : a.groups == 1 ? team : team / (unsigned)a.groups;
     const int64_t off = !in ? 0 : (int64_t)(team - (unsigned)row * (unsigned)a.groups) * a.d;   // of the group
@@ -243,8 +261,8 @@ rows_kernel(const __grid_constant__ Args a) {
         if (!NORM || !a.weight) {
 #pragma unroll
             for (int j = 0; j < V; ++j) w[j] = 1.0f;
-        } else if (a.w32) load<A, V, false>(static_cast<const float*>(a.weight) + at(i), a.d - at(i), w);
-        else load<A, V, false>(static_cast<const T*>(a.weight) + at(i), a.d - at(i), w);
+        } else if (a.w32) load<A, V, false>(static_cast<const float*>(a.weight) + at(i), d - at(i), w);
+        else load<A, V, false>(static_cast<const T*>(a.weight) + at(i), d - at(i), w);
     };
     float sum = 0.0f, top = 0.0f;
     auto gather = [&](float by) {
@@ -262,22 +280,21 @@ rows_kernel(const __grid_constant__ Args a) {
         }
     };
     gather(1.0f);
-    const float2 st = team_sum_max<TPR>(sum, top, red[0]);
+    const float2 st = team_sum_max<TEAM>(sum, top, red[0]);
     float top_g = st.y, by = 1.0f;
     double sum_sq = st.x;
-    if (NORM && !(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
+    const bool odd = NORM && !(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f);
+    if (NORM && __any_sync(~0u, odd)) {                    // the teams of a warp go together
         // near the ends of float32's range: again with h scaled by a power of two
         float hm = 0.0f;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) hm = max_nan(hm, fabsf(h[i]));
-        const float htop = team_sum_max<TPR>(0.0f, hm, red[1]).y;
-        if (htop > 0.0f && is_finite(htop)) {
-            by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
-            gather(by);
-            const float2 s2 = team_sum_max<TPR>(sum, top, red[2]);
-            top_g = s2.y;
-            sum_sq = s2.x;
-        }
+        const float htop = team_sum_max<TEAM>(0.0f, hm, red[1]).y;
+        if (odd && htop > 0.0f && is_finite(htop)) by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
+        gather(by);
+        const float2 s2 = team_sum_max<TEAM>(sum, top, red[2]);
+        top_g = s2.y;
+        sum_sq = s2.x;
     }
     const Quant quant(top_g);
     const bool wanted = in && slot >= 0 && (NORM || slot < a.nslots);
@@ -342,7 +359,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
             if (NORM) sum = __fmaf_rn(h, h, sum);
             top = max_nan(top, fabsf(h * w_of(j)));
         }
-        return team_sum_max<LONG_THREADS>(sum, top, r);
+        return team_sum_max<0>(sum, top, r);
     };
     const float2 st = gather(1.0f, red[0]);
     float top_g = st.y, by = 1.0f, step = top_g / 127.0f;
@@ -351,7 +368,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
         if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
             float hm = 0.0f;
             for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max_nan(hm, fabsf(h_of(j)));
-            const float htop = team_sum_max<LONG_THREADS>(0.0f, hm, red[1]).y;
+            const float htop = team_sum_max<0>(0.0f, hm, red[1]).y;
             if (htop > 0.0f && is_finite(htop)) {
                 by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
                 const float2 s2 = gather(by, red[2]);
@@ -371,26 +388,33 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
         a.scale[to * a.groups + g] = !is_finite(top_g) ? __uint_as_float(0x7fffffffu) : top_g > 0.0f ? step : 0.0f;
 }
 
-template <class T, class R, int TPR, int EPT, Access A, bool NORM>
+template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 void launch_team(const Args& a, cudaStream_t s) {
-    constexpr unsigned per = block_of(TPR) / TPR;
-    rows_kernel<T, R, TPR, EPT, A, NORM><<<(a.teams - 1) / per + 1, block_of(TPR), 0, s>>>(a);
+    constexpr unsigned per = SHARED_BLOCK / TEAM;
+    rows_kernel<T, R, TEAM, EPT, A, NORM><<<(a.teams - 1) / per + 1, SHARED_BLOCK, 0, s>>>(a);
 }
-// The smallest team whose registers hold a row.
+template <class T, class R, int EPT, Access A, bool NORM>
+void launch_block(const Args& a, cudaStream_t s) {
+    rows_kernel<T, R, 0, EPT, A, NORM><<<a.teams, (a.d - 1) / EPT / 32 * 32 + 32, 0, s>>>(a);
+}
+// Many rows: the smallest team whose registers hold a row at 32 values a thread (at 16 and 8 the instructions spent on
+// a row bind: 65536 x 4096 in bfloat16 took 441 us with 16, 303 us with 32). Few rows, which leave SMs idle: as few
+// values a thread as a block allows (1 x 4096: 3.4 us with 16, 3.8 us with 32).
 template <class T, class R, Access A, bool NORM>
 void launch_rows(const Args& a, cudaStream_t s) {
     const int d = a.d;
-    if (!NORM && d <= 32) launch_team<T, R, 4, 8, A, NORM>(a, s);
+    if (d > 32 * MOST_THREADS) long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
+    else if (a.teams <= 2 * SMS && d > 256 && d <= 8 * MOST_THREADS) launch_block<T, R, 8, A, NORM>(a, s);
+    else if (a.teams <= 2 * SMS && d > 256 && d <= 16 * MOST_THREADS) launch_block<T, R, 16, A, NORM>(a, s);
+    else if (!NORM && d <= 16) launch_team<T, R, 2, 8, A, NORM>(a, s);
+    else if (!NORM && d <= 32) launch_team<T, R, 4, 8, A, NORM>(a, s);
     else if (!NORM && d <= 64) launch_team<T, R, 4, 16, A, NORM>(a, s);
-    else if (!NORM && d <= 128) launch_team<T, R, 8, 16, A, NORM>(a, s);
-    else if (d <= 256) launch_team<T, R, NORM ? 32 : 16, NORM ? 8 : 16, A, NORM>(a, s);
+    else if (d <= 128) launch_team<T, R, 8, 16, A, NORM>(a, s);
+    else if (d <= 256) launch_team<T, R, 16, 16, A, NORM>(a, s);
     else if (d <= 512) launch_team<T, R, 32, 16, A, NORM>(a, s);
-    else if (d <= 1024) launch_team<T, R, 32, 32, A, NORM>(a, s);
-    else if (d <= 2048) launch_team<T, R, 64, 32, A, NORM>(a, s);
-    else if (d <= 4096) launch_team<T, R, 128, 32, A, NORM>(a, s);
-    else if (d <= 8192) launch_team<T, R, 256, 32, A, NORM>(a, s);
-    else if (d <= 16384) launch_team<T, R, 512, 32, A, NORM>(a, s);
-    else long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
+    else if (A == SINGLE && d <= 16 * MOST_THREADS) launch_block<T, R, 16, A, NORM>(a, s);   // 32 addresses do not fit
+    else if (A != SINGLE && d <= 1024) launch_team<T, R, 32, 32, A, NORM>(a, s);
+    else launch_block<T, R, 32, A, NORM>(a, s);
 }
 
 bool on_bytes(const void* p, int64_t ld, int size, int rows_of, int64_t rows) {
@@ -403,19 +427,31 @@ template <class T, int V>
 struct alignas(V * sizeof(T)) Piece {
     T v[V];
 };
-// Value i of a piece as a float: the byte + 128 as the low bits of 2^23, less
-// 2^23 + 128 (exact); half the cost of a conversion.
+// V bytes of a row, and value i of them as a float: the byte + 128 as the low bits
+// of 2^23, less 2^23 + 128 (exact); half the cost of a conversion.
 template <int V>
-__device__ __forceinline__ float byte_float(const Piece<int8_t, V>& b, int i) {
-    if constexpr (V == 1) return (float)b.v[0];
-    else {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(b.v)[i / 4] ^ 0x80808080u;
-        return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + i % 4)) - 8388736.0f;
+struct Bytes {
+    uint32_t w[(V + 3) / 4];
+    __device__ __forceinline__ void load(const int8_t* p) {
+        if constexpr (V == 16) {
+            const uint4 v = load16(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else if constexpr (V == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[1] = v.y;
+        } else if constexpr (V == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint8_t*>(p);
+        }
     }
-}
+    __device__ __forceinline__ float value(int i) const {
+        return __uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4B000000u, 0x7440 + i % 4)) - 8388736.0f;
+    }
+};
 
 template <class T, int V, int U>
-__global__ void __launch_bounds__(256, U == 1 ? 6 : 4)
+__global__ void __launch_bounds__(256, U == 1 ? 8 : V <= 4 ? 5 : 6)
 read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
             const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
             int gdim, int dim) {
@@ -431,15 +467,15 @@ read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__
         fac[u] = scale + (there ? slot * groups : 0);
     }
     for (int j = (blockIdx.y * tpr + threadIdx.x % tpr) * V; j < dim; j += (int)gridDim.y * tpr * V) {
-        Piece<int8_t, V> b[U];
+        Bytes<V> b[U];
         float sc[U];
         const unsigned g = groups == 1 ? 0u : (unsigned)j / (unsigned)gdim;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             sc[u] = 0.0f;
-            b[u] = Piece<int8_t, V>{};
+            b[u] = Bytes<V>{};
             if (from[u]) {
-                b[u] = *reinterpret_cast<const Piece<int8_t, V>*>(from[u] + j);
+                b[u].load(from[u] + j);
                 sc[u] = fac[u][g];
             }
         }
@@ -450,7 +486,7 @@ read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__
             T* o = out + row * ldo + j;
             alignas(32) T v[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) from_float(&v[i], sc[u] * byte_float(b[u], i));
+            for (int i = 0; i < V; ++i) from_float(&v[i], sc[u] * b[u].value(i));
             if constexpr (V * sizeof(T) == 32) {
                 const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
                 asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -470,12 +506,13 @@ bool try_read(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, c
                   !on_bytes(out->data, out->ld, sizeof(T), V * (int)sizeof(T), out->rows)))
         return false;
     const int tpr = std::min(256, next_pow2((int)ceil_div(dim, V)));
-    // two rows a thread once that leaves every SM eight blocks
-    const int U = out->rows >= (int64_t)2 * 8 * SMS * (256 / tpr) ? 2 : 1;
+    // several rows a thread once that leaves every SM eight blocks
+    constexpr int MORE = V <= 4 ? 4 : 2;
+    const int U = out->rows >= (int64_t)MORE * 8 * SMS * (256 / tpr) ? MORE : 1;
     const int64_t blocks = ceil_div(out->rows, 256 / tpr * U);
     if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
-    const dim3 grid((unsigned)blocks, (unsigned)(U == 2 ? 1 : std::min<int64_t>(65535, ceil_div(dim, tpr * V))));
-    (U == 2 ? read_kernel<T, V, 2> : read_kernel<T, V, 1>)<<<grid, 256, 0, s>>>(
+    const dim3 grid((unsigned)blocks, (unsigned)(U > 1 ? 1 : std::min<int64_t>(65535, ceil_div(dim, tpr * V))));
+    (U > 1 ? read_kernel<T, V, MORE> : read_kernel<T, V, 1>)<<<grid, 256, 0, s>>>(
         c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows, tpr, c->groups, gdim, dim);
     return true;
 }
