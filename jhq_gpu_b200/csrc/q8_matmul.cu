@@ -210,8 +210,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // finishing TN / S of the tokens. 32-bit integer sums are exact, so the split
 // changes no output.
 constexpr int BM = 128, BK = 128;
-constexpr int LOADERS = 256;                               // threads that load where TMA cannot
-constexpr int panel_threads(bool tma) { return 64 + (tma ? 128 : LOADERS); }
+constexpr int LOADERS = 256;                               // threads of the epilogue, which load where TMA cannot
+constexpr int PANEL_THREADS = 64 + LOADERS;
 
 template <int TN>
 struct Panel {
@@ -272,41 +272,39 @@ __device__ __forceinline__ void load_rows(const Rows8& m, int64_t row0, int r0, 
 }
 
 // Adds the S CTAs' sums of this thread's channel for the rank's TN / S tokens and
-// finishes them; `part` is the shared address of the channel's first sum. The
-// reads of eight tokens from all CTAs are in flight together.
+// finishes them, the two warps of a quarter every other batch; `part` is the shared
+// address of the channel's first sum, sx holds the scales of the rank's tokens. The
+// reads of up to eight tokens from all CTAs are in flight together.
 template <int TN, int S>
-__device__ __forceinline__ void join(const Epilogue& e, uint32_t part, int rank, int64_t t0, const float* sx, int n,
-                                     float sw, float b) {
-    constexpr int PER = TN / S, R = PER < 8 ? PER : 8;
+__device__ __forceinline__ void join(const Epilogue& e, uint32_t part, int rank, int half, int64_t t0, const float* sx,
+                                     int n, float sw, float b) {
+    constexpr int PER = TN / S, R = PER < 16 ? (PER + 1) / 2 : 8;
     uint32_t from[S];
 #pragma unroll
     for (int p = 0; p < S; ++p) from[p] = map_to(part, p);
-#pragma unroll 1
-    for (int i = 0; i < PER; i += R) {
-        const int c = rank * PER + i;
-        if (t0 + c >= e.T) break;
+#pragma unroll
+    for (int k = 0; k < (PER + 2 * R - 1) / (2 * R); ++k) {
+        const int i = (2 * k + half) * R, c = rank * PER + i;
+        if (i >= PER || t0 + c >= e.T) break;
         int v[S][R];
 #pragma unroll
         for (int p = 0; p < S; ++p)
 #pragma unroll
             for (int j = 0; j < R; ++j)
                 asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[p][j]) : "r"(from[p] + (c + j) * BM * 4));
-        float scale = sx[0];
-#pragma unroll
-        for (int k = 1; k < (TN + 31) / 32; ++k) scale = c / 32 == k ? sx[k] : scale;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             int sum = 0;
 #pragma unroll
             for (int p = 0; p < S; ++p) sum += v[p][j];
-            const float f = (float)sum * __shfl_sync(~0u, scale, (c + j) % 32) * sw;
+            const float f = (float)sum * __shfl_sync(~0u, sx[2 * k * R / 32], (i + j) % 32) * sw;
             if (t0 + c + j < e.T && n < e.N) store_out(e, t0 + c + j, n, e.bias ? f + b : f);
         }
     }
 }
 
 template <int TN, bool TMA>
-__global__ void __launch_bounds__(panel_threads(TMA), 1)
+__global__ void __launch_bounds__(PANEL_THREADS, 1)
 panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, Rows8 w,
              Rows8 x, int K, int S, int ttiles, Epilogue e) {
     using P = Panel<TN>;
@@ -403,12 +401,17 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         }
     }
 
-    const int q4 = warp & 3, row = q4 * 32 + lane, n = m0 + row;
-    const bool epi = warp >= 2 && warp < 6;
-    const float sw = epi && n < e.N ? e.sw[n] : 0.0f, b = epi && n < e.N && e.bias ? e.bias[n] : 0.0f;
-    constexpr int NSX = (TN + 31) / 32;
-    float sx[NSX];
-    if (epi) get_scales<NSX>(e, t0, sx);
+    // epilogue: warp w and w + 4 share a TMEM lane quarter and split the tokens
+    constexpr int HALF = TN == 16 ? 16 : TN / 2;
+    const int q4 = warp & 3, row = q4 * 32 + lane, n = m0 + row, half = warp >= 6 ? 1 : 0;
+    const bool epi = warp >= 2 && half * HALF < TN;
+    const int c0 = half * HALF;
+    const bool mine = warp >= 2 && n < e.N;
+    const float sw = mine ? e.sw[n] : 0.0f, b = mine && e.bias ? e.bias[n] : 0.0f;
+    constexpr int NSX = (HALF + 31) / 32;
+    float sx[NSX];                                         // of this CTA's tokens c0 .. (S = 1), or of those it finishes
+    const int per = TN / S;
+    if (warp >= 2) get_scales<NSX>(e, t0 + (S == 1 ? c0 : rank * per), sx);
     bool ok = true;
     __syncwarp();
     if (epi) {
@@ -416,32 +419,32 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         ok = __all_sync(~0u, ok && !abort);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16) + c0;
     if (S == 1) {
         if (epi && ok) {
 #pragma unroll
-            for (int c = 0; c < TN; c += 16) {
+            for (int c = 0; c < HALF; c += 16) {
                 int r[16];
                 tmem_ld16(r, lanes + c);
-                put16(e, r, t0 + c, sx[c / 32], c % 32, n, sw, b);
+                put16(e, r, t0 + c0 + c, sx[c / 32], c % 32, n, sw, b);
             }
         }
     } else {
         int* part = reinterpret_cast<int*>(smem);          // [TN][128]: every MMA has read its stage
         if (epi && ok) {
 #pragma unroll
-            for (int c = 0; c < TN; c += 16) {
+            for (int c = 0; c < HALF; c += 16) {
                 int r[16];
                 tmem_ld16(r, lanes + c);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) part[(c + j) * BM + row] = r[j];
+                for (int j = 0; j < 16; ++j) part[(c0 + c + j) * BM + row] = r[j];
             }
         }
         cluster_sync();
-        if (epi && ok) {
-            if (S == 2) join<TN, 2>(e, base + row * 4, rank, t0, sx, n, sw, b);
-            else if (S == 4) join<TN, 4>(e, base + row * 4, rank, t0, sx, n, sw, b);
-            else join<TN, 8>(e, base + row * 4, rank, t0, sx, n, sw, b);
+        if (warp >= 2 && ok) {
+            if (S == 2) join<TN, 2>(e, base + row * 4, rank, half, t0, sx, n, sw, b);
+            else if (S == 4) join<TN, 4>(e, base + row * 4, rank, half, t0, sx, n, sw, b);
+            else join<TN, 8>(e, base + row * 4, rank, half, t0, sx, n, sw, b);
         }
         cluster_sync();                                    // no CTA leaves while its sums are read
     }
@@ -744,47 +747,63 @@ CUtensorMap make_map(const jhq_q8_rows* r, int box_rows) {
 constexpr int SMS = 148;
 
 template <int TN, bool TMA>
-void launch_panels(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaStream_t s) {
+void panel_attributes() {
     static std::atomic<uint64_t> done{0};
     once_per_device(done, [] {
         JHQ_CUDA(cudaFuncSetAttribute(panel_kernel<TN, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Panel<TN>::SMEM));
     });
-    const int64_t ttiles = ceil_div(x->rows, TN), tiles = ttiles * ceil_div(w->rows, BM);
-    const int nkb = (int)ceil_div(x->dim, BK);
-    int S = 1;                     
-    while (S < 8 && tiles * S * 2 <= SMS && nkb >= 4 * S) S *= 2;
-    if (tiles * S > INT32_MAX) fail(JHQ_EINVAL, "q8_matmul: too many rows");
-    CUtensorMap mw{}, mx{};
-    if (TMA) { mw = make_map(w, BM); mx = make_map(x, TN); }
+}
+
+template <int TN, bool TMA>
+cudaLaunchConfig_t panel_config(int64_t blocks, int S, cudaLaunchAttribute* at, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * S));
-    cfg.blockDim = dim3(panel_threads(TMA));
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(PANEL_THREADS);
     cfg.dynamicSmemBytes = Panel<TN>::SMEM;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)S;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
+    return cfg;
+}
+
+// CTAs of panels that run at once in clusters of S (one an SM; a cluster stays within a GPC, so fewer with large S).
+int panel_capacity(int S) {
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> held[4];                       // of the last device asked; all B200s alike but for spare SMs
+    once_per_device(done, [] {
+        panel_attributes<64, true>();
+        for (int k = 0; k < 4; ++k) {
+            cudaLaunchAttribute at[1];
+            const cudaLaunchConfig_t cfg = panel_config<64, true>(SMS << k, 1 << k, at, nullptr);
+            int n = 0;
+            JHQ_CUDA(cudaOccupancyMaxActiveClusters(&n, panel_kernel<64, true>, &cfg));
+            held[k] = std::max(1, n << k);
+        }
+    });
+    return held[S == 1 ? 0 : S == 2 ? 1 : S == 4 ? 2 : 3];
+}
+
+template <int TN, bool TMA>
+void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, int S, const Epilogue& e, cudaStream_t s) {
+    panel_attributes<TN, TMA>();
+    const int64_t ttiles = ceil_div(x->rows, TN), blocks = ttiles * ceil_div(w->rows, BM) * S;
+    if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_matmul: too many rows");
+    CUtensorMap mw{}, mx{};
+    if (TMA) { mw = make_map(w, BM); mx = make_map(x, TN); }
+    cudaLaunchAttribute at[1];
+    const cudaLaunchConfig_t cfg = panel_config<TN, TMA>(blocks, S, at, s);
     JHQ_CUDA(cudaLaunchKernelEx(&cfg, panel_kernel<TN, TMA>, mw, mx, Rows8{w->q, w->ld, w->rows},
                                 Rows8{x->q, x->ld, x->rows}, (int)x->dim, S, (int)ttiles, e));
 }
-
 template <bool TMA>
-void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaStream_t s) {
-    if (x->rows <= 16) launch_panels<16, TMA>(x, w, e, s);
-    else if (x->rows <= 32) launch_panels<32, TMA>(x, w, e, s);
-    else if (x->rows <= 64) launch_panels<64, TMA>(x, w, e, s);
-    else launch_panels<128, TMA>(x, w, e, s);
-}
-
-// Microseconds of the busiest pair with tiles of 256 tokens by tn channels, from what a K block and a tile cost when
-// measured alone: 0.20 and 2.0 with 128 channels, 0.275 and 3.3 with 256. The narrow tile wins where the wide one leaves
-// pairs idle (512 x 1024 x 1024: 7.3 against 9.4 us), the wide one elsewhere (32768 x 8192 x 8192: 1293 against 1862 us).
-double pair_cost(const jhq_q8_rows* x, const jhq_q8_rows* w, int tn, double block, double tile) {
-    const int64_t tiles = ceil_div(x->rows, 2 * BM) * ceil_div(w->rows, tn);
-    return (double)ceil_div(tiles, SMS / 2) * ((double)ceil_div(x->dim, BK) * block + tile);
+void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, int TN, int S, const Epilogue& e, cudaStream_t s) {
+    if (TN == 16) panels<16, TMA>(x, w, S, e, s);
+    else if (TN == 32) panels<32, TMA>(x, w, S, e, s);
+    else if (TN == 64) panels<64, TMA>(x, w, S, e, s);
+    else panels<128, TMA>(x, w, S, e, s);
 }
 
 template <int TN>
@@ -797,6 +816,43 @@ void pairs(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaSt
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(SMS / 2, mt * nt);
     pair_kernel<TN><<<grid, PAIR_THREADS, Pair<TN>::SMEM, s>>>(make_map(x, BM), make_map(w, TN / 2), (int)x->dim,
                                                                (int)mt, (int)nt, e);
+}
+
+// Which kernel, tile and split: the least of the microseconds that these costs, fitted to timings of single launches
+// in a graph, give. A K block of 128 bytes takes 0.195 us in a panel of any width (issue of copies and MMAs) and in a pair
+// 0.20 us with 128 channels, 0.272 us with 256 (the MMAs); the rest is launch, filling the ring and the epilogue. Examples,
+// best panel / pair of 128 / pair of 256: 256 x 1024 x 4096 8.0 / 11.6 / 15.4 us; 512 x 1024 x 1024 6.2 / 6.9 / 8.9;
+// 256 x 4096 x 4096 11.4 / 12.0 / 15.8; 8192 x 4096 x 4096 236 / 112 / 88.
+struct Plan {
+    int tile, split;                                       // split 0: pairs
+    double us;
+};
+Plan plan(const jhq_q8_rows* x, const jhq_q8_rows* w) {
+    const int64_t nkb = ceil_div(x->dim, BK), mt = ceil_div(w->rows, BM);
+    Plan best{256, 0, 0.0};
+    for (int tn : {256, 128}) {
+        const double block = tn == 256 ? 0.272 : 0.20, first = tn == 256 ? 6.7 : 5.2, least = tn == 256 ? 6.2 : 3.2;
+        const int64_t waves = ceil_div(ceil_div(x->rows, 2 * BM) * ceil_div(w->rows, tn), SMS / 2);
+        const double us = first + nkb * block + (double)(waves - 1) * std::max(nkb * block, least);
+        if (tn == 256 || us < best.us) best = {tn, 0, us};
+    }
+    if (x->rows > 2048) return best;
+    for (int tn = 16; tn <= 128; tn *= 2) {
+        for (int S = 1; S <= 8 && 2 * S <= std::max<int64_t>(nkb, 2); S *= 2) {
+            const int64_t waves = ceil_div(ceil_div(x->rows, tn) * mt * S, panel_capacity(S));
+            const double us = (double)waves * ((double)ceil_div(nkb, S) * 0.195 + (tn == 16 ? 4.0 : tn == 32 ? 4.6 : tn == 64 ? 5.4 : 7.0) + (S > 1 ? 0.8 : 0.0));
+            if (us < best.us) best = {tn, S, us};
+        }
+        if (tn >= x->rows) break;
+    }
+    return best;
+}
+// Rows that TMA cannot fetch: the loader threads bind, who bring 128 + tile rows for 128 x tile products.
+Plan plan_unaligned(const jhq_q8_rows* x, const jhq_q8_rows* w) {
+    Plan p{x->rows <= 16 ? 16 : x->rows <= 32 ? 32 : x->rows <= 64 ? 64 : 128, 1, 0.0};
+    const int64_t tiles = ceil_div(x->rows, p.tile) * ceil_div(w->rows, BM), nkb = ceil_div(x->dim, BK);
+    while (p.split < 8 && nkb >= 4 * p.split && tiles * p.split * 2 <= panel_capacity(2 * p.split)) p.split *= 2;
+    return p;
 }
 
 }  // namespace
@@ -821,9 +877,11 @@ void q8_matmul(const jhq_q8_rows* x, const jhq_q8_rows* w, const jhq_view* bias,
     const Epilogue e{x->scale, w->scale, bias ? (const float*)bias->data : nullptr, out->data, out->ld,
                      x->rows, (int)w->rows, out->type,
                      (uintptr_t)out->data % 16 == 0 && out->ld % (out->type == JHQ_F32 ? 4 : 8) == 0};
-    if (!on_boundaries(x) || !on_boundaries(w)) panels<false>(x, w, e, s);
-    else if (x->rows <= 128) panels<true>(x, w, e, s);
-    else if (pair_cost(x, w, 128, 0.20, 2.0) < pair_cost(x, w, 256, 0.275, 3.3)) pairs<128>(x, w, e, s);
+    const bool tma = on_boundaries(x) && on_boundaries(w);
+    const Plan p = tma ? plan(x, w) : plan_unaligned(x, w);
+    if (!tma) panels<false>(x, w, p.tile, p.split, e, s);
+    else if (p.split) panels<true>(x, w, p.tile, p.split, e, s);
+    else if (p.tile == 128) pairs<128>(x, w, e, s);
     else pairs<256>(x, w, e, s);
     JHQ_LAUNCH_CHECK();
     count_launch();

@@ -19,19 +19,30 @@ import jhq_gpu_b200 as _J
 F32, F16, BF16 = range(3)
 _TYPES = {"float32": F32, "float16": F16, "bfloat16": BF16,
           "torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+_PAIRS = set()                                            # dtypes of values and scales that were found right
+
+
+def _kind(dtype) -> int:
+    kind = _TYPES.get(str(dtype))
+    if kind is None:
+        raise ValueError(f"View: float32, float16 or bfloat16 is needed, got {dtype}")
+    _TYPES[dtype] = kind                                  # the next look finds the dtype itself
+    return kind
 
 
 def _shape(t, what: str):
     """rows, columns and row stride of a 2-D (or, as one row, 1-D) tensor."""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 1:
-        shape, stride = (1, shape[0]), (shape[0] * stride[0], stride[0])
-    if len(shape) != 2:
+    if len(shape) == 2:
+        rows, cols = shape
+        ld, step = stride
+    elif len(shape) == 1:
+        rows, cols, ld, step = 1, shape[0], 0, stride[0]
+    else:
         raise ValueError(f"{what}: a 2-D tensor is needed, got {len(shape)} dimensions")
-    rows, cols = shape
-    if cols > 1 and stride[1] != 1:
-        raise ValueError(f"{what}: the values of a row must follow one another (stride {stride[1]})")
-    return rows, cols, stride[0] if rows > 1 else cols
+    if step != 1 and cols > 1:
+        raise ValueError(f"{what}: the values of a row must follow one another (stride {step})")
+    return rows, cols, ld if rows > 1 else cols
 
 
 class View(C.Structure):
@@ -41,11 +52,8 @@ class View(C.Structure):
 
     @classmethod
     def of(cls, t) -> "View":
-        kind = _TYPES.get(str(t.dtype))
-        if kind is None:
-            raise ValueError(f"View: float32, float16 or bfloat16 is needed, got {t.dtype}")
-        rows, cols, ld = _shape(t, "View")
-        return cls(t.data_ptr(), rows, cols, ld, kind)
+        kind = _TYPES.get(t.dtype)
+        return cls(t.data_ptr(), *_shape(t, "View"), _kind(t.dtype) if kind is None else kind)
 
 
 class Q8Rows(C.Structure):
@@ -56,8 +64,10 @@ class Q8Rows(C.Structure):
     @classmethod
     def of(cls, q, scale, groups: int = 1) -> "Q8Rows":
         """q: (rows, dim) int8; scale: rows * groups float32, packed."""
-        if str(q.dtype) not in ("torch.int8", "int8") or str(scale.dtype) not in ("torch.float32", "float32"):
-            raise ValueError(f"Q8Rows: int8 values and float32 scales are needed, got {q.dtype} and {scale.dtype}")
+        if (q.dtype, scale.dtype) not in _PAIRS:
+            if str(q.dtype) not in ("torch.int8", "int8") or str(scale.dtype) not in ("torch.float32", "float32"):
+                raise ValueError(f"Q8Rows: int8 values and float32 scales are needed, got {q.dtype} and {scale.dtype}")
+            _PAIRS.add((q.dtype, scale.dtype))
         rows, dim, ld = _shape(q, "Q8Rows")
         if scale.numel() != rows * groups or not scale.is_contiguous():
             raise ValueError(f"Q8Rows: {rows} x {groups} packed scales are needed")
