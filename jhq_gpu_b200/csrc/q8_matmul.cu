@@ -225,49 +225,83 @@ struct Panel {
 struct Rows8 {                       // operand rows for the loader threads
     const int8_t* p;
     int64_t ld, rows;
+    const int8_t* end;               // behind the last row's last byte
 };
 
-// One warp copies bytes k .. k + 127 of R rows (row0 + r0, + r0 + step, ...) into
-// swizzled 128-byte rows of shared memory, zeros beyond the rows' ends. Rows
-// begin at any address: a lane reads an aligned word and shifts it together with
-// its neighbour's (lane 31 reads one more). Only words that lie inside the row are
-// read whole; the bytes of those that straddle its ends are read one by one. The
-// loads of all R rows are in flight together.
-template <int R>
-__device__ __forceinline__ void load_rows(const Rows8& m, int64_t row0, int r0, int step, int k, int K, uint32_t dst,
-                                          int lane) {
-    uint32_t lo[R], ex[R];
-    int off[R];
-    const bool edge = k == 0 || k + BK + 4 > K;            // the block touches an end of its rows
+__device__ __forceinline__ uint4 load16_if(bool ok, const int8_t* p) {
+    uint4 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                 "@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok));
+    return v;
+}
+// The 16 bytes at p, zeros outside [first, end): byte by byte.
+__device__ __noinline__ uint4 load16_edge(const int8_t* p, const int8_t* first, const int8_t* end) {
+    uint32_t w[4] = {};
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+        if (p + i >= first && p + i < end) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The loader warps copy bytes k .. k + 127 of BM rows of w (from w0) and TN rows of
+// x (from x0) into swizzled 128-byte rows of shared memory, zeros beyond the rows'
+// ends. Rows begin at any address: eight lanes take a row, each the aligned 16 bytes
+// that its output begins in, and shift them together with the next lane's (the
+// eighth reads one piece more). A piece may reach into a neighbouring row or the space
+// between rows, whose bytes are cut off, but not out of the matrix: the few
+// that straddle its first or last byte are read byte by byte. All pieces of a warp
+// are in flight together.
+template <int TN>
+__device__ __forceinline__ void load_stage(const Rows8& w, const Rows8& x, int64_t w0, int64_t x0, int k, int K,
+                                           uint32_t dst, int lw, int lane) {
+    constexpr int STEP = LOADERS / 8, NW = BM / STEP, NX = (TN + STEP - 1) / STEP, N = NW + NX;
+    const int c = lane & 7, r0 = lw * 4 + lane / 8;
+    uint4 v[N], ex[N];
+    int off[N];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t row = row0 + r0 + i * step;
-        const bool in = row < m.rows;
+    for (int b = 0; b < N; ++b) {
+        const Rows8& m = b < NW ? w : x;
+        const int r = r0 + STEP * (b < NW ? b : b - NW);
+        const int64_t row = (b < NW ? w0 : x0) + r;
+        const bool in = row < m.rows && (b < NW || r < TN);
         const int8_t* at = m.p + (in ? row : 0) * m.ld + k;
-        off[i] = (int)((uintptr_t)at & 3);
-        const int pos = k - off[i] + 4 * lane;             // of the word in the row
-        const int8_t* a = at - off[i] + 4 * lane;
-        lo[i] = in && pos >= 0 && pos + 4 <= K ? *reinterpret_cast<const uint32_t*>(a) : 0u;
-        ex[i] = in && lane == 31 && pos + 8 <= K ? *reinterpret_cast<const uint32_t*>(a + 4) : 0u;
-        if (edge) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const bool b0 = in && (pos < 0 || pos + 4 > K) && pos + c >= 0 && pos + c < K;
-                const bool b1 = in && lane == 31 && pos + 8 > K && pos + 4 + c < K;
-                const uint32_t v0 = b0 ? (uint32_t)(uint8_t)a[c] : 0u, v1 = b1 ? (uint32_t)(uint8_t)a[4 + c] : 0u;
-                lo[i] |= v0 << (8 * c);
-                ex[i] |= v1 << (8 * c);
-            }
-        }
+        off[b] = (int)((uintptr_t)at & 15);
+        const int8_t* piece = at - off[b] + 16 * c;
+        const int left = K - k + off[b] - 16 * c;          // of the row, from the piece's first byte
+        const bool ok = in && left > 0, more = in && c == 7 && off[b] > 0 && left > 16;
+        const bool whole = piece >= m.p && piece + 16 <= m.end, whole2 = piece + 32 <= m.end;
+        v[b] = load16_if(ok && whole, piece);
+        ex[b] = load16_if(more && whole2, piece + 16);
+        if (ok && !whole) v[b] = load16_edge(piece, m.p, m.end);
+        if (more && !whole2) ex[b] = load16_edge(piece + 16, m.p, m.end);
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        uint32_t hi = __shfl_down_sync(~0u, lo[i], 1);
-        if (lane == 31) hi = ex[i];
-        const int r = r0 + i * step;
-        asm volatile("st.shared.b32 [%0], %1;"
-                     :: "r"(dst + r * 128 + ((4 * lane) ^ ((r & 7) << 4))), "r"(__funnelshift_r(lo[i], hi, 8 * off[i]))
-                     : "memory");
+    for (int b = 0; b < N; ++b) {
+        const int r = r0 + STEP * (b < NW ? b : b - NW);
+        uint32_t a[8] = {v[b].x, v[b].y, v[b].z, v[b].w};
+        a[4] = __shfl_down_sync(~0u, v[b].x, 1);
+        a[5] = __shfl_down_sync(~0u, v[b].y, 1);
+        a[6] = __shfl_down_sync(~0u, v[b].z, 1);
+        a[7] = __shfl_down_sync(~0u, v[b].w, 1);
+        if (c == 7) { a[4] = ex[b].x; a[5] = ex[b].y; a[6] = ex[b].z; a[7] = ex[b].w; }
+        const bool two = off[b] & 8, one = off[b] & 4;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) a[i] = two ? a[i + 2] : a[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) a[i] = one ? a[i + 1] : a[i];
+        const int sh = 8 * (off[b] & 3), left = K - k - 16 * c;
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[i] = __funnelshift_r(a[i], a[i + 1], sh);
+            const int bytes = left - 4 * i;                // of the row, in this word
+            if (bytes < 4) o[i] = bytes > 0 ? o[i] & ((1u << (8 * bytes)) - 1) : 0u;
+        }
+        if (b < NW || r < TN)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
+                         :: "r"(dst + (b < NW ? 0 : BM * BK) + r * 128 + ((c ^ (r & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                         : "memory");
     }
 }
 
@@ -391,11 +425,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             if (it >= P::STAGES && !__all_sync(~0u, mbar_wait(empty0 + 8 * s, (it / P::STAGES - 1) & 1, &abort))) break;
             const uint32_t dst = base + s * P::STAGE;
             const int k = (kb0 + it) * BK;
-            constexpr int LW = LOADERS / 32, R = 8, RX = TN / LW < R ? TN / LW : R;
-#pragma unroll 1
-            for (int r = lw; r < BM; r += LW * R) load_rows<R>(w, m0, r, LW, k, K, dst, lane);
-#pragma unroll 1
-            for (int r = lw; r < TN; r += LW * RX) load_rows<RX>(x, t0, r, LW, k, K, dst + BM * BK, lane);
+            load_stage<TN>(w, x, m0, t0, k, K, dst, lw, lane);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(full0 + 8 * s) : "memory");
         }
@@ -746,6 +776,8 @@ CUtensorMap make_map(const jhq_q8_rows* r, int box_rows) {
 
 constexpr int SMS = 148;
 
+Rows8 rows8(const jhq_q8_rows* r) { return {r->q, r->ld, r->rows, r->q + (r->rows - 1) * r->ld + r->dim}; }
+
 template <int TN, bool TMA>
 void panel_attributes() {
     static std::atomic<uint64_t> done{0};
@@ -795,8 +827,7 @@ void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, int S, const Epilogue& e
     if (TMA) { mw = make_map(w, BM); mx = make_map(x, TN); }
     cudaLaunchAttribute at[1];
     const cudaLaunchConfig_t cfg = panel_config<TN, TMA>(blocks, S, at, s);
-    JHQ_CUDA(cudaLaunchKernelEx(&cfg, panel_kernel<TN, TMA>, mw, mx, Rows8{w->q, w->ld, w->rows},
-                                Rows8{x->q, x->ld, x->rows}, (int)x->dim, S, (int)ttiles, e));
+    JHQ_CUDA(cudaLaunchKernelEx(&cfg, panel_kernel<TN, TMA>, mw, mx, rows8(w), rows8(x), (int)x->dim, S, (int)ttiles, e));
 }
 template <bool TMA>
 void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, int TN, int S, const Epilogue& e, cudaStream_t s) {

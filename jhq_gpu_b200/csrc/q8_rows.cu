@@ -72,20 +72,20 @@ __device__ __forceinline__ void load_if(bool ok, const uint4* p, uint4& v) {
     if (STREAM)
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
                      "@p ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
-                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok) : "memory");
+                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok));
     else
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
                      "@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
-                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok) : "memory");
+                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok));
 }
 __device__ __forceinline__ float load_if(bool ok, const float* p) {
     uint32_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(v) : "l"(p), "r"((int)ok) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(v) : "l"(p), "r"((int)ok));
     return __uint_as_float(v);
 }
 __device__ __forceinline__ uint16_t load_if_16(bool ok, const void* p) {
     uint16_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}" : "=&h"(v) : "l"(p), "r"((int)ok) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}" : "=&h"(v) : "l"(p), "r"((int)ok));
     return v;
 }
 __device__ __forceinline__ float load_if(bool ok, const __half* p) { return __half2float(__ushort_as_half(load_if_16(ok, p))); }
@@ -439,10 +439,8 @@ struct Bytes {
         } else if constexpr (V == 8) {
             const uint2 v = *reinterpret_cast<const uint2*>(p);
             w[0] = v.x; w[1] = v.y;
-        } else if constexpr (V == 4) {
-            w[0] = *reinterpret_cast<const uint32_t*>(p);
         } else {
-            w[0] = *reinterpret_cast<const uint8_t*>(p);
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
     }
     __device__ __forceinline__ float value(int i) const {
@@ -499,11 +497,58 @@ read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__
     }
 }
 
+// Rows at odd addresses or of odd groups: EACH values a thread, tpr apart, so that
+// accesses stay side by side.
+constexpr int EACH = 8;
+template <class T>
+__global__ void __launch_bounds__(256)
+read_odd_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
+                const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
+                int gdim, uint32_t inverse, int dim) {
+    const int64_t row = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+    const int64_t slot = row >= rows ? -1 : slots ? slots[row] : row;
+    const bool there = slot >= 0 && slot < nslots;
+    q += there ? slot * ldq : 0;
+    scale += there ? slot * groups : 0;
+    out += row * ldo;
+    for (int j0 = blockIdx.y * tpr * EACH + threadIdx.x % tpr; j0 < dim; j0 += (int)gridDim.y * tpr * EACH) {
+        int b[EACH];
+        float sc[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int j = j0 + i * tpr;
+            // j / gdim, by floor(2^32 / gdim): at most one too small
+            uint32_t g = groups == 1 ? 0u : __umulhi((uint32_t)j, inverse);
+            if (groups != 1 && (uint32_t)j - g * gdim >= (uint32_t)gdim) ++g;
+            const bool ok = there && j < dim;
+            b[i] = ok ? (int)q[j] : 0;
+            sc[i] = ok ? scale[g] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int j = j0 + i * tpr;
+            if (row < rows && j < dim) from_float(out + j, sc[i] * (float)b[i]);
+        }
+    }
+}
+
+template <class T>
+void read_odd(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, cudaStream_t s) {
+    const int gdim = (int)(c->dim / c->groups), dim = (int)c->dim;
+    const int tpr = std::max(32, std::min(256, next_pow2((int)ceil_div(dim, EACH))));
+    const int64_t blocks = ceil_div(out->rows, 256 / tpr);
+    if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
+    const uint32_t inverse = gdim == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / gdim);
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(65535, ceil_div(dim, tpr * EACH)));
+    read_odd_kernel<T><<<grid, 256, 0, s>>>(c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows, tpr,
+                                            c->groups, gdim, inverse, dim);
+}
+
 template <class T, int V>
 bool try_read(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, cudaStream_t s) {
     const int gdim = (int)(c->dim / c->groups), dim = (int)c->dim;
-    if (V > 1 && (gdim % V || !on_bytes(c->q, c->ld, 1, V, c->rows) ||
-                  !on_bytes(out->data, out->ld, sizeof(T), V * (int)sizeof(T), out->rows)))
+    if (gdim % V || !on_bytes(c->q, c->ld, 1, V, c->rows) ||
+        !on_bytes(out->data, out->ld, sizeof(T), V * (int)sizeof(T), out->rows))
         return false;
     const int tpr = std::min(256, next_pow2((int)ceil_div(dim, V)));
     // several rows a thread once that leaves every SM eight blocks
@@ -632,7 +677,7 @@ void q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out
         using T = decltype(t);
         if (!try_read<T, 32 / (int)sizeof(T)>(cache, slots, out, s) && !try_read<T, 8>(cache, slots, out, s) &&
             !try_read<T, 4>(cache, slots, out, s))
-            try_read<T, 1>(cache, slots, out, s);
+            read_odd<T>(cache, slots, out, s);
     });
     JHQ_LAUNCH_CHECK();
     count_launch();
