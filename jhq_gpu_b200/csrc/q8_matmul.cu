@@ -211,7 +211,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // changes no output.
 constexpr int BM = 128, BK = 128;
 constexpr int LOADERS = 256;                               // threads of the epilogue, which load where TMA cannot
-constexpr int PANEL_THREADS = 64 + LOADERS;
+constexpr int LOAD_GROUPS = 2;                             // as many again, which load every other stage
+constexpr int panel_threads(bool tma) { return 64 + LOADERS * (tma ? 1 : LOAD_GROUPS); }
 
 template <int TN>
 struct Panel {
@@ -338,7 +339,7 @@ __device__ __forceinline__ void join(const Epilogue& e, uint32_t part, int rank,
 }
 
 template <int TN, bool TMA>
-__global__ void __launch_bounds__(PANEL_THREADS, 1)
+__global__ void __launch_bounds__(panel_threads(TMA), 1)
 panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, Rows8 w,
              Rows8 x, int K, int S, int ttiles, Epilogue e) {
     using P = Panel<TN>;
@@ -419,10 +420,10 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                          :: "r"(done) : "memory");
         }
     } else if (!TMA) {                                     // the other warps fill the stages
-        const int lw = warp - 2;
-        for (int it = 0; it < nk; ++it) {
+        const int group = (warp - 2) / (LOADERS / 32), lw = (warp - 2) % (LOADERS / 32);
+        for (int it = group; it < nk; it += LOAD_GROUPS) {
             const int s = it % P::STAGES;
-            if (it >= P::STAGES && !__all_sync(~0u, mbar_wait(empty0 + 8 * s, (it / P::STAGES - 1) & 1, &abort))) break;
+            if (it >= P::STAGES && !warp_wait(empty0 + 8 * s, (it / P::STAGES - 1) & 1, &abort)) break;
             const uint32_t dst = base + s * P::STAGE;
             const int k = (kb0 + it) * BK;
             load_stage<TN>(w, x, m0, t0, k, K, dst, lw, lane);
@@ -434,14 +435,14 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     // epilogue: warp w and w + 4 share a TMEM lane quarter and split the tokens
     constexpr int HALF = TN == 16 ? 16 : TN / 2;
     const int q4 = warp & 3, row = q4 * 32 + lane, n = m0 + row, half = warp >= 6 ? 1 : 0;
-    const bool epi = warp >= 2 && half * HALF < TN;
+    const bool epi = warp >= 2 && warp < 10 && half * HALF < TN;
     const int c0 = half * HALF;
-    const bool mine = warp >= 2 && n < e.N;
+    const bool mine = warp >= 2 && warp < 10 && n < e.N;
     const float sw = mine ? e.sw[n] : 0.0f, b = mine && e.bias ? e.bias[n] : 0.0f;
     constexpr int NSX = (HALF + 31) / 32;
     float sx[NSX];                                         // of this CTA's tokens c0 .. (S = 1), or of those it finishes
     const int per = TN / S;
-    if (warp >= 2) get_scales<NSX>(e, t0 + (S == 1 ? c0 : rank * per), sx);
+    if (warp >= 2 && warp < 10) get_scales<NSX>(e, t0 + (S == 1 ? c0 : rank * per), sx);
     bool ok = true;
     __syncwarp();
     if (epi) {
@@ -471,7 +472,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             }
         }
         cluster_sync();
-        if (warp >= 2 && ok) {
+        if (warp >= 2 && warp < 10 && ok) {
             if (S == 2) join<TN, 2>(e, base + row * 4, rank, half, t0, sx, n, sw, b);
             else if (S == 4) join<TN, 4>(e, base + row * 4, rank, half, t0, sx, n, sw, b);
             else join<TN, 8>(e, base + row * 4, rank, half, t0, sx, n, sw, b);
@@ -790,7 +791,7 @@ template <int TN, bool TMA>
 cudaLaunchConfig_t panel_config(int64_t blocks, int S, cudaLaunchAttribute* at, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(PANEL_THREADS);
+    cfg.blockDim = dim3(panel_threads(TMA));
     cfg.dynamicSmemBytes = Panel<TN>::SMEM;
     cfg.stream = s;
     at[0].id = cudaLaunchAttributeClusterDimension;

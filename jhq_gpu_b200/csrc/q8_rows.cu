@@ -78,24 +78,12 @@ __device__ __forceinline__ void load_if(bool ok, const uint4* p, uint4& v) {
                      "@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
                      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)ok));
 }
-__device__ __forceinline__ float load_if(bool ok, const float* p) {
-    uint32_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(v) : "l"(p), "r"((int)ok));
-    return __uint_as_float(v);
-}
-__device__ __forceinline__ uint16_t load_if_16(bool ok, const void* p) {
-    uint16_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}" : "=&h"(v) : "l"(p), "r"((int)ok));
-    return v;
-}
-__device__ __forceinline__ float load_if(bool ok, const __half* p) { return __half2float(__ushort_as_half(load_if_16(ok, p))); }
-__device__ __forceinline__ float load_if(bool ok, const __nv_bfloat16* p) { return __bfloat162float(__ushort_as_bfloat16(load_if_16(ok, p))); }
 
 template <Access A, int V, bool STREAM, class T>
 __device__ __forceinline__ void load(const T* p, int left, float* out) {
     constexpr int B = V * (int)sizeof(T);
     if constexpr (A == SINGLE) {
-        out[0] = load_if(left > 0, p);
+        out[0] = left > 0 ? to_float(*p) : 0.0f;
     } else {
         if (A == RAGGED && left > 0 && left < V) {
 #pragma unroll
@@ -176,15 +164,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// Sum and maximum over a team: TEAM lanes of a warp, or the block (TEAM = 0).
+// Sum and maximum over a team: up to 32 lanes of a warp, or the block (of TEAM
+// threads, or of any number: TEAM = 0).
 template <int TEAM>
 __device__ __forceinline__ float2 team_sum_max(float sum, float top, float2* red) {
 #pragma unroll
-    for (int o = (TEAM ? TEAM : 32) / 2; o; o >>= 1) {
+    for (int o = (TEAM && TEAM < 32 ? TEAM : 32) / 2; o; o >>= 1) {
         sum += __shfl_xor_sync(~0u, sum, o);
         top = max_nan(top, __shfl_xor_sync(~0u, top, o));
     }
-    if (TEAM == 0) {
+    if (TEAM == 0 || TEAM > 32) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         if (lane == 0) red[warp] = make_float2(sum, top);
         __syncthreads();
@@ -224,15 +213,18 @@ constexpr int SMS = 148;
 // every output is written once. Bound by those bytes, as long as a thread has
 // enough values that the instructions spent on a row and not on a value (addresses,
 // the team's reductions, the reciprocal) stay few. Short groups share a warp, rows
-// to 1024 values have a warp, longer ones a block (TEAM = 0). Registers are held to
+// to 1024 values have a warp, longer ones a block, of as many threads as they need
+// (TEAM = 0) or, for single values, whose addresses then differ by constants, of TEAM
+// (20000 x 1001 in bfloat16, packed: 100 instructions a value without that). Registers are held to
 // what lets an SM hold 768 threads with 32 values each, 1024 with fewer.
 constexpr int SHARED_BLOCK = 128, MOST_THREADS = 512;
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_constant__ Args a) {
     constexpr int V = A == SINGLE ? 1 : 16 / (int)sizeof(T), NV = EPT / V;
     __shared__ float2 red[3][32];
-    const int TPR = TEAM ? TEAM : (int)blockDim.x, me = TEAM ? threadIdx.x % TEAM : threadIdx.x;
-    const unsigned team = TEAM ? blockIdx.x * (SHARED_BLOCK / (TEAM ? TEAM : 1)) + threadIdx.x / (TEAM ? TEAM : 1) : blockIdx.x;
+    constexpr bool SHARED = TEAM && TEAM <= 32;            // blocks of several teams
+    const int TPR = TEAM ? TEAM : (int)blockDim.x, me = SHARED ? threadIdx.x % TPR : threadIdx.x;
+    const unsigned team = SHARED ? blockIdx.x * (SHARED_BLOCK / TPR) + threadIdx.x / TPR : blockIdx.x;
     const bool in = team < a.teams;                        // else the team only keeps the warp's shuffles company
     const int64_t row = !in ? 0 : a.groups == 1 ? team : team / (unsigned)a.groups;
     const int64_t off = !in ? 0 : (int64_t)(team - (unsigned)row * (unsigned)a.groups) * a.d;   // of the group
@@ -390,31 +382,39 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
 
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 void launch_team(const Args& a, cudaStream_t s) {
-    constexpr unsigned per = SHARED_BLOCK / TEAM;
-    rows_kernel<T, R, TEAM, EPT, A, NORM><<<(a.teams - 1) / per + 1, SHARED_BLOCK, 0, s>>>(a);
+    constexpr unsigned per = TEAM <= 32 ? SHARED_BLOCK / TEAM : 1;
+    rows_kernel<T, R, TEAM, EPT, A, NORM><<<(a.teams - 1) / per + 1, TEAM <= 32 ? SHARED_BLOCK : TEAM, 0, s>>>(a);
 }
 template <class T, class R, int EPT, Access A, bool NORM>
 void launch_block(const Args& a, cudaStream_t s) {
     rows_kernel<T, R, 0, EPT, A, NORM><<<a.teams, (a.d - 1) / EPT / 32 * 32 + 32, 0, s>>>(a);
 }
 // Many rows: the smallest team whose registers hold a row at 32 values a thread (at 16 and 8 the instructions spent on
-// a row bind: 65536 x 4096 in bfloat16 took 441 us with 16, 303 us with 32). Few rows, which leave SMs idle: as few
-// values a thread as a block allows (1 x 4096: 3.4 us with 16, 3.8 us with 32).
+// a row bind: 65536 x 4096 in bfloat16 took 441 us with 16, 303 us with 32), at 16 single values, whose registers
+// 32 do not fit. Few rows, which leave SMs idle: as few values a thread as a block allows (1 x 4096: 3.4 us with 16,
+// 3.8 us with 32).
 template <class T, class R, Access A, bool NORM>
 void launch_rows(const Args& a, cudaStream_t s) {
     const int d = a.d;
-    if (d > 32 * MOST_THREADS) long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
-    else if (a.teams <= 2 * SMS && d > 256 && d <= 8 * MOST_THREADS) launch_block<T, R, 8, A, NORM>(a, s);
-    else if (a.teams <= 2 * SMS && d > 256 && d <= 16 * MOST_THREADS) launch_block<T, R, 16, A, NORM>(a, s);
-    else if (!NORM && d <= 16) launch_team<T, R, 2, 8, A, NORM>(a, s);
-    else if (!NORM && d <= 32) launch_team<T, R, 4, 8, A, NORM>(a, s);
-    else if (!NORM && d <= 64) launch_team<T, R, 4, 16, A, NORM>(a, s);
-    else if (d <= 128) launch_team<T, R, 8, 16, A, NORM>(a, s);
-    else if (d <= 256) launch_team<T, R, 16, 16, A, NORM>(a, s);
-    else if (d <= 512) launch_team<T, R, 32, 16, A, NORM>(a, s);
-    else if (A == SINGLE && d <= 16 * MOST_THREADS) launch_block<T, R, 16, A, NORM>(a, s);   // 32 addresses do not fit
-    else if (A != SINGLE && d <= 1024) launch_team<T, R, 32, 32, A, NORM>(a, s);
-    else launch_block<T, R, 32, A, NORM>(a, s);
+    const bool few = a.teams <= 2 * SMS && d > 256;
+    if (!NORM && d <= 16) return launch_team<T, R, 2, 8, A, NORM>(a, s);
+    if (!NORM && d <= 32) return launch_team<T, R, 4, 8, A, NORM>(a, s);
+    if (!NORM && d <= 64) return launch_team<T, R, 4, 16, A, NORM>(a, s);
+    if (d <= 128) return launch_team<T, R, 8, 16, A, NORM>(a, s);
+    if (d <= 256) return launch_team<T, R, 16, 16, A, NORM>(a, s);
+    if (few && d <= 8 * MOST_THREADS) return launch_block<T, R, 8, A, NORM>(a, s);
+    if (few && d <= 16 * MOST_THREADS) return launch_block<T, R, 16, A, NORM>(a, s);
+    if (d <= 512) return launch_team<T, R, 32, 16, A, NORM>(a, s);
+    if constexpr (A == SINGLE) {
+        if (d <= 1024) return launch_team<T, R, 64, 16, A, NORM>(a, s);
+        if (d <= 2048) return launch_team<T, R, 128, 16, A, NORM>(a, s);
+        if (d <= 4096) return launch_team<T, R, 256, 16, A, NORM>(a, s);
+        if (d <= 8192) return launch_team<T, R, 512, 16, A, NORM>(a, s);
+    } else {
+        if (d <= 1024) return launch_team<T, R, 32, 32, A, NORM>(a, s);
+        if (d <= 32 * MOST_THREADS) return launch_block<T, R, 32, A, NORM>(a, s);
+    }
+    long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
 }
 
 bool on_bytes(const void* p, int64_t ld, int size, int rows_of, int64_t rows) {
