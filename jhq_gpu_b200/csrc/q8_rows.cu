@@ -497,51 +497,82 @@ read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__
     }
 }
 
-// Rows at odd addresses or of odd groups: EACH values a thread, tpr apart, so that
-// accesses stay side by side.
-constexpr int EACH = 8;
-template <class T>
+// The four bytes at p (any address) of a buffer [first, end): from the two aligned words that hold them, where these lie
+// inside, else byte by byte, zeros outside.
+__device__ __noinline__ uint32_t word_edge(const int8_t* p, const int8_t* first, const int8_t* end) {
+    uint32_t v = 0;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i)
+        if (p + i >= first && p + i < end) v |= (uint32_t)(uint8_t)p[i] << (8 * i);
+    return v;
+}
+
+// Rows at odd addresses or of odd groups: a thread takes the V values of an aligned
+// 32 bytes of output (the first and last piece of a row: of what the row has of
+// them) and gathers their bytes from aligned words. WALK: groups shorter than a piece.
+template <class T, bool WALK>
 __global__ void __launch_bounds__(256)
-read_odd_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
-                const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
-                int gdim, uint32_t inverse, int dim) {
+read_odd_kernel(const int8_t* __restrict__ q, int64_t ldq, const int8_t* __restrict__ end, const float* __restrict__ scale,
+                int64_t nslots, const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr,
+                int groups, int gdim, int dim) {
+    constexpr int V = 32 / (int)sizeof(T);
     const int64_t row = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
-    const int64_t slot = row >= rows ? -1 : slots ? slots[row] : row;
+    if (row >= rows) return;
+    const int64_t slot = slots ? slots[row] : row;
     const bool there = slot >= 0 && slot < nslots;
-    q += there ? slot * ldq : 0;
-    scale += there ? slot * groups : 0;
-    out += row * ldo;
-    for (int j0 = blockIdx.y * tpr * EACH + threadIdx.x % tpr; j0 < dim; j0 += (int)gridDim.y * tpr * EACH) {
-        int b[EACH];
-        float sc[EACH];
+    const int8_t* const from = q + (there ? slot * ldq : 0);
+    const float* const fac = scale + (there ? slot * groups : 0);
+    T* const o = out + row * ldo;
+    const int skew = (int)((uintptr_t)o % 32 / sizeof(T));             // values of the first piece before the row
+    for (int j0 = (blockIdx.y * tpr + threadIdx.x % tpr) * V - skew; j0 < dim; j0 += (int)gridDim.y * tpr * V) {
+        uint32_t w[V / 4 + 1];
+        const int8_t* const p = from + j0;
+        const int off = (int)((uintptr_t)p & 3);
+        const int8_t* const a = p - off;
+        const bool inside = j0 >= 0 && a >= q && a + V + 4 <= end;      // whole words of the buffer
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int j = j0 + i * tpr;
-            // j / gdim, by floor(2^32 / gdim): at most one too small
-            uint32_t g = groups == 1 ? 0u : __umulhi((uint32_t)j, inverse);
-            if (groups != 1 && (uint32_t)j - g * gdim >= (uint32_t)gdim) ++g;
-            const bool ok = there && j < dim;
-            b[i] = ok ? (int)q[j] : 0;
-            sc[i] = ok ? scale[g] : 0.0f;
+        for (int i = 0; i <= V / 4; ++i) w[i] = there && inside ? reinterpret_cast<const uint32_t*>(a)[i] : 0u;
+        const int first = max(j0, 0), g = groups == 1 ? 0 : (int)((unsigned)first / (unsigned)gdim);
+        const int turn = groups == 1 ? dim : (g + 1) * gdim;            // where the next group begins
+        const float sc = there ? fac[g] : 0.0f, sc1 = there && turn < min(j0 + V, dim) ? fac[g + 1] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * off);
+        if (there && !inside) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) w[i] = word_edge(p + 4 * i, from, from + dim);
         }
+        alignas(16) T v[V];
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int j = j0 + i * tpr;
-            if (row < rows && j < dim) from_float(out + j, sc[i] * (float)b[i]);
+        for (int i = 0; i < V; ++i) {
+            const int j = j0 + i;
+            float f = j < turn ? sc : sc1;
+            if (WALK && there && j >= turn && j < dim) f = fac[(unsigned)j / (unsigned)gdim];
+            const float b = __uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4B000000u, 0x7440 + i % 4)) - 8388736.0f;
+            from_float(&v[i], there ? f * b : 0.0f);
+        }
+        if (j0 >= 0 && j0 + V <= dim) {
+            reinterpret_cast<uint4*>(o + j0)[0] = reinterpret_cast<const uint4*>(v)[0];
+            reinterpret_cast<uint4*>(o + j0)[1] = reinterpret_cast<const uint4*>(v)[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (j0 + i >= 0 && j0 + i < dim) o[j0 + i] = v[i];
         }
     }
 }
 
 template <class T>
 void read_odd(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, cudaStream_t s) {
+    constexpr int V = 32 / (int)sizeof(T);
     const int gdim = (int)(c->dim / c->groups), dim = (int)c->dim;
-    const int tpr = std::max(32, std::min(256, next_pow2((int)ceil_div(dim, EACH))));
+    const int64_t pieces = ceil_div(dim, V) + 1;
+    const int tpr = std::min(256, next_pow2((int)std::min<int64_t>(256, pieces)));
     const int64_t blocks = ceil_div(out->rows, 256 / tpr);
     if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
-    const uint32_t inverse = gdim == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / gdim);
-    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(65535, ceil_div(dim, tpr * EACH)));
-    read_odd_kernel<T><<<grid, 256, 0, s>>>(c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows, tpr,
-                                            c->groups, gdim, inverse, dim);
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(65535, ceil_div(pieces, tpr)));
+    (gdim < V && c->groups > 1 ? read_odd_kernel<T, true> : read_odd_kernel<T, false>)<<<grid, 256, 0, s>>>(
+        c->q, c->ld, c->rows ? c->q + (c->rows - 1) * c->ld + dim : c->q, c->scale, c->rows, slots, (T*)out->data, out->ld,
+        out->rows, tpr, c->groups, gdim, dim);
 }
 
 template <class T, int V>
