@@ -419,6 +419,19 @@ def test_launches_are_counted(jhq):
     assert jhq.kernel_launches() >= n + 2
 
 
+@gpu
+def test_example_finds_the_queries_items():
+    """A query's embedding has a cosine of about 0.99 with its item's and one of at most about 6 / sqrt(128) = 0.53 with any
+    of 5000 others: the first result is its item unless a kernel is wrong."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "q8_embedding_search.py")
+    spec = importlib.util.spec_from_file_location("q8_embedding_search", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main(n=5000, nq=200) >= 0.99
+
+
 # ---- refusals (no GPU is touched) -----------------------------------------------------------------------------
 
 def _v(jhq, rows=4, cols=64, ld=None, kind=0, data=4096):
