@@ -1,0 +1,35 @@
+// q8_launch.cuh — launches of the 8-bit row kernels, which follow one another
+// closely (norm, product, cache), as programmatic dependents: a kernel's blocks
+// may start while the last blocks of the one before it in the stream finish, and
+// set up what touches no memory that those may still write or read; before_memory()
+// then waits until they are done and their writes are visible.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "jhq_common.h"
+
+namespace jhq {
+
+__device__ __forceinline__ void before_memory() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Once every block has called this (or ended), the next kernel's blocks may start.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... P, class... A>
+void launch_q8(void (*kernel)(P...), dim3 grid, unsigned block, size_t smem, int cluster, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    JHQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
+}  // namespace jhq

@@ -20,6 +20,7 @@
 
 #include "kernels.cuh"
 #include "q8.h"
+#include "q8_launch.cuh"
 
 namespace jhq {
 
@@ -378,8 +379,14 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         mbar_init(done, 1);
         abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (TMA)                                           // the ring is filled before anything else is set up
+        let_next_start();
+        if (TMA) {                                         // the ring is filled before anything else is set up
+            for (int it = 0; it < min(nk, P::STAGES); ++it)   // only into L2, where it can turn out to be any kernel's
+                asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
+                             :: "l"((uint64_t)&map_w), "r"((kb0 + it) * BK), "r"(m0) : "memory");
+            before_memory();
             for (int it = 0; it < min(nk, P::STAGES); ++it) load(it, it);
+        }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -390,6 +397,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
+    before_memory();
 
     if (warp == 0) {
         if (TMA && elect_one()) {
@@ -599,6 +607,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
         mbar_init(drain, 1);
         abort = 0;
+        let_next_start();
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -611,6 +620,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
+    before_memory();
 
     auto tile_at = [&](int64_t i, int64_t& t0, int& n0) {  // the first token and channel of tile i
         const int64_t group = i / ((int64_t)RASTER * nt), r = i - group * RASTER * nt;
@@ -787,21 +797,6 @@ void panel_attributes() {
     });
 }
 
-template <int TN, bool TMA>
-cudaLaunchConfig_t panel_config(int64_t blocks, int S, cudaLaunchAttribute* at, cudaStream_t s) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(panel_threads(TMA));
-    cfg.dynamicSmemBytes = Panel<TN>::SMEM;
-    cfg.stream = s;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)S;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cfg;
-}
-
 // CTAs of panels that run at once in clusters of S (one an SM; a cluster stays within a GPC, so fewer with large S).
 int panel_capacity(int S) {
     static std::atomic<uint64_t> done{0};
@@ -810,7 +805,15 @@ int panel_capacity(int S) {
         panel_attributes<64, true>();
         for (int k = 0; k < 4; ++k) {
             cudaLaunchAttribute at[1];
-            const cudaLaunchConfig_t cfg = panel_config<64, true>(SMS << k, 1 << k, at, nullptr);
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 1u << k;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(SMS << k);
+            cfg.blockDim = dim3(panel_threads(true));
+            cfg.dynamicSmemBytes = Panel<64>::SMEM;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
             int n = 0;
             JHQ_CUDA(cudaOccupancyMaxActiveClusters(&n, panel_kernel<64, true>, &cfg));
             held[k] = std::max(1, n << k);
@@ -826,9 +829,8 @@ void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, int S, const Epilogue& e
     if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_matmul: too many rows");
     CUtensorMap mw{}, mx{};
     if (TMA) { mw = make_map(w, BM); mx = make_map(x, TN); }
-    cudaLaunchAttribute at[1];
-    const cudaLaunchConfig_t cfg = panel_config<TN, TMA>(blocks, S, at, s);
-    JHQ_CUDA(cudaLaunchKernelEx(&cfg, panel_kernel<TN, TMA>, mw, mx, rows8(w), rows8(x), (int)x->dim, S, (int)ttiles, e));
+    launch_q8(panel_kernel<TN, TMA>, dim3((unsigned)blocks), panel_threads(TMA), Panel<TN>::SMEM, S, s, mw, mx, rows8(w),
+              rows8(x), (int)x->dim, S, (int)ttiles, e);
 }
 template <bool TMA>
 void panels(const jhq_q8_rows* x, const jhq_q8_rows* w, int TN, int S, const Epilogue& e, cudaStream_t s) {
@@ -846,8 +848,8 @@ void pairs(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaSt
     });
     const int64_t mt = ceil_div(x->rows, 2 * BM), nt = ceil_div(w->rows, TN);
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(SMS / 2, mt * nt);
-    pair_kernel<TN><<<grid, PAIR_THREADS, Pair<TN>::SMEM, s>>>(make_map(x, BM), make_map(w, TN / 2), (int)x->dim,
-                                                               (int)mt, (int)nt, e);
+    launch_q8(pair_kernel<TN>, dim3(grid), PAIR_THREADS, Pair<TN>::SMEM, 0, s, make_map(x, BM), make_map(w, TN / 2),
+              (int)x->dim, (int)mt, (int)nt, e);
 }
 
 // Which kernel, tile and split: the least of the microseconds that these costs, fitted to timings of single launches

@@ -15,6 +15,7 @@
 
 #include "kernels.cuh"
 #include "q8.h"
+#include "q8_launch.cuh"
 
 namespace jhq {
 
@@ -221,6 +222,8 @@ constexpr int SHARED_BLOCK = 128, MOST_THREADS = 512;
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_constant__ Args a) {
     constexpr int V = A == SINGLE ? 1 : 16 / (int)sizeof(T), NV = EPT / V;
+    let_next_start();
+    before_memory();
     __shared__ float2 red[3][32];
     constexpr bool SHARED = TEAM && TEAM <= 32;            // blocks of several teams
     const int TPR = TEAM ? TEAM : (int)blockDim.x, me = SHARED ? threadIdx.x % TPR : threadIdx.x;
@@ -326,6 +329,8 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
 constexpr int LONG_THREADS = 1024;
 template <class T, class R, bool NORM>
 __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_constant__ Args a) {
+    let_next_start();
+    before_memory();
     __shared__ float2 red[3][32];
     const int64_t row = a.groups == 1 ? blockIdx.x : blockIdx.x / (unsigned)a.groups;
     const int g = a.groups == 1 ? 0 : (int)(blockIdx.x % (unsigned)a.groups);
@@ -383,11 +388,11 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 void launch_team(const Args& a, cudaStream_t s) {
     constexpr unsigned per = TEAM <= 32 ? SHARED_BLOCK / TEAM : 1;
-    rows_kernel<T, R, TEAM, EPT, A, NORM><<<(a.teams - 1) / per + 1, TEAM <= 32 ? SHARED_BLOCK : TEAM, 0, s>>>(a);
+    launch_q8(rows_kernel<T, R, TEAM, EPT, A, NORM>, dim3((a.teams - 1) / per + 1), TEAM <= 32 ? SHARED_BLOCK : TEAM, 0, 0, s, a);
 }
 template <class T, class R, int EPT, Access A, bool NORM>
 void launch_block(const Args& a, cudaStream_t s) {
-    rows_kernel<T, R, 0, EPT, A, NORM><<<a.teams, (a.d - 1) / EPT / 32 * 32 + 32, 0, s>>>(a);
+    launch_q8(rows_kernel<T, R, 0, EPT, A, NORM>, dim3(a.teams), (a.d - 1) / EPT / 32 * 32 + 32, 0, 0, s, a);
 }
 // Many rows: the smallest team whose registers hold a row at 32 values a thread (at 16 and 8 the instructions spent on
 // a row bind: 65536 x 4096 in bfloat16 took 441 us with 16, 303 us with 32), at 16 single values, whose registers
@@ -414,7 +419,7 @@ void launch_rows(const Args& a, cudaStream_t s) {
         if (d <= 1024) return launch_team<T, R, 32, 32, A, NORM>(a, s);
         if (d <= 32 * MOST_THREADS) return launch_block<T, R, 32, A, NORM>(a, s);
     }
-    long_rows_kernel<T, R, NORM><<<a.teams, LONG_THREADS, 0, s>>>(a);
+    launch_q8(long_rows_kernel<T, R, NORM>, dim3(a.teams), LONG_THREADS, 0, 0, s, a);
 }
 
 bool on_bytes(const void* p, int64_t ld, int size, int rows_of, int64_t rows) {
@@ -453,6 +458,8 @@ __global__ void __launch_bounds__(256, U == 1 ? 8 : V <= 4 ? 5 : 6)
 read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
             const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
             int gdim, int dim) {
+    let_next_start();
+    before_memory();
     const int per = 256 / tpr;
     const int64_t row0 = (int64_t)blockIdx.x * per * U + threadIdx.x / tpr;
     const int8_t* from[U];
@@ -516,6 +523,8 @@ read_odd_kernel(const int8_t* __restrict__ q, int64_t ldq, const int8_t* __restr
                 int64_t nslots, const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr,
                 int groups, int gdim, int dim) {
     constexpr int V = 32 / (int)sizeof(T);
+    let_next_start();
+    before_memory();
     const int64_t row = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
     if (row >= rows) return;
     const int64_t slot = slots ? slots[row] : row;
@@ -570,8 +579,7 @@ void read_odd(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, c
     const int64_t blocks = ceil_div(out->rows, 256 / tpr);
     if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
     const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(65535, ceil_div(pieces, tpr)));
-    (gdim < V && c->groups > 1 ? read_odd_kernel<T, true> : read_odd_kernel<T, false>)<<<grid, 256, 0, s>>>(
-        c->q, c->ld, c->rows ? c->q + (c->rows - 1) * c->ld + dim : c->q, c->scale, c->rows, slots, (T*)out->data, out->ld,
+    launch_q8(gdim < V && c->groups > 1 ? read_odd_kernel<T, true> : read_odd_kernel<T, false>, grid, 256, 0, 0, s, c->q, c->ld, c->rows ? c->q + (c->rows - 1) * c->ld + dim : c->q, c->scale, c->rows, slots, (T*)out->data, out->ld,
         out->rows, tpr, c->groups, gdim, dim);
 }
 
@@ -588,8 +596,7 @@ bool try_read(const jhq_q8_rows* c, const int64_t* slots, const jhq_view* out, c
     const int64_t blocks = ceil_div(out->rows, 256 / tpr * U);
     if (blocks > INT32_MAX) fail(JHQ_EINVAL, "q8_read: too many rows");
     const dim3 grid((unsigned)blocks, (unsigned)(U > 1 ? 1 : std::min<int64_t>(65535, ceil_div(dim, tpr * V))));
-    (U > 1 ? read_kernel<T, V, MORE> : read_kernel<T, V, 1>)<<<grid, 256, 0, s>>>(
-        c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows, tpr, c->groups, gdim, dim);
+    launch_q8(U > 1 ? read_kernel<T, V, MORE> : read_kernel<T, V, 1>, grid, 256, 0, 0, s, c->q, c->ld, c->scale, c->rows, slots, (T*)out->data, out->ld, out->rows, tpr, c->groups, gdim, dim);
     return true;
 }
 

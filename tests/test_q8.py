@@ -410,6 +410,32 @@ def test_on_a_side_stream_and_in_a_graph(jhq):
 
 
 @gpu
+@pytest.mark.parametrize("t,d,n", [(1, 1024, 512), (40, 4096, 1000), (700, 640, 300), (3000, 512, 1024), (33, 999, 130)])
+def test_calls_wait_for_one_another(jhq, t, d, n):
+    """Kernels start while the one before them ends: a chain over shared buffers gives what it gives call by call."""
+    w, ws = _q8(87, n, d, (d + 15) // 16 * 16)
+    q, scale = _q8(88, t, d, (d + 15) // 16 * 16)
+    h, back, kept = torch.empty(t, n, device="cuda"), torch.empty(t, n, device="cuda"), _q8(89, t, n)
+
+    def chain(x, wait):
+        rows, cache = jhq.Q8Rows.of(q, scale), jhq.Q8Rows.of(*kept)
+        for call in (lambda: jhq.q8_rms_norm(jhq.View.of(x), rows, stream=_stream()),
+                     lambda: jhq.q8_matmul(rows, jhq.Q8Rows.of(w, ws), jhq.View.of(h), stream=_stream()),
+                     lambda: jhq.q8_write(jhq.View.of(h), cache, stream=_stream()),
+                     lambda: jhq.q8_read(cache, jhq.View.of(back), stream=_stream())):
+            call()
+            if wait:
+                torch.cuda.synchronize()
+        return back.clone()
+
+    xs = [_randn(200 + i, t, d) * (i + 1) for i in range(12)]
+    want = [chain(x, True) for x in xs]
+    for _ in range(4):
+        got = [chain(x, False) for x in xs]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
 def test_launches_are_counted(jhq):
     x = _randn(91, 4, 64)
     q, s = torch.empty(4, 64, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
