@@ -56,9 +56,9 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(10000u) : "memory");   // may sleep so many ns
     return ok != 0;
 }
 
@@ -201,6 +201,18 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     bool ok = true;
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort);
     return __all_sync(~0u, ok);
+}
+// The wait of a panel's epilogue warps, through the whole of its products: the first
+// one's lane 0 polls, the others sleep at a barrier. (With all eight polling, the barrier
+// operations of the producers and the MMA thread took 0.16 us a K block.)
+__device__ __forceinline__ bool epilogue_wait(uint32_t bar, uint32_t parity, volatile int* abort, bool polls, int threads) {
+    bool ok = true;
+    if (polls && (threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort);
+    __syncwarp();
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((int)ok), "r"(threads) : "memory");
+    return all != 0;
 }
 
 // ---- panels: few tokens, or rows at any address ------------------------------
@@ -359,21 +371,30 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     const int nkb = (K + BK - 1) / BK;                     // K blocks; this CTA's: kb0 .. kb0 + nk - 1
     const int kb0 = (int)((int64_t)nkb * rank / S), nk = (int)((int64_t)nkb * (rank + 1) / S) - kb0;
 
-    auto load = [&](int it, int s) {                       // block kb0 + it into stage s (one thread)
-        const uint32_t fb = full0 + 8 * s, dst = base + s * P::STAGE;
-        mbar_expect(fb, P::STAGE);
-        const int k = (kb0 + it) * BK;
+    // Block kb0 + it of one operand into stage s (one thread; two share the copies).
+    auto load = [&](int it, int s, bool of_w) {
+        const uint32_t fb = full0 + 8 * s, dst = base + s * P::STAGE + (of_w ? 0 : BM * BK);
+        mbar_expect(fb, of_w ? BM * BK : TN * BK);
         asm volatile(
             "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-            :: "r"(dst), "l"((uint64_t)&map_w), "r"(k), "r"(m0), "r"(fb) : "memory");
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-            :: "r"(dst + BM * BK), "l"((uint64_t)&map_x), "r"(k), "r"((int)t0), "r"(fb) : "memory");
+            :: "r"(dst), "l"((uint64_t)(of_w ? &map_w : &map_x)), "r"((kb0 + it) * BK), "r"(of_w ? m0 : (int)t0), "r"(fb)
+            : "memory");
+    };
+    auto produce = [&](int it, bool of_w) {                // blocks it, it + 1, ...; it = 0, or those of the ring are done
+        const uint32_t odd = it == 0 ? 1u : 0u;            // the ring's second round waits for the first phase
+        Ring<P::STAGES> r;                                 // begins at a multiple of STAGES, or ends there
+        for (; it < nk; ++it, r.next()) {
+            if (it >= P::STAGES && !mbar_wait(empty0 + 8 * r.s, r.phase ^ odd, &abort)) break;
+            load(it, r.s, of_w);
+        }
+        if (abort)                                         // copies in flight land before the CTA ends
+            for (int j = max(it - P::STAGES, 0); j < it; ++j)
+                mbar_wait(full0 + 8 * (j % P::STAGES), (j / P::STAGES) & 1, nullptr);
     };
 
     if (tid == 0) {
         for (int i = 0; i < P::STAGES; ++i) {
-            mbar_init(full0 + 8 * i, TMA ? 1 : LOADERS);
+            mbar_init(full0 + 8 * i, TMA ? 2 : LOADERS);
             mbar_init(empty0 + 8 * i, 1);
         }
         mbar_init(done, 1);
@@ -385,7 +406,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                 asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
                              :: "l"((uint64_t)&map_w), "r"((kb0 + it) * BK), "r"(m0) : "memory");
             before_memory();
-            for (int it = 0; it < min(nk, P::STAGES); ++it) load(it, it);
+            for (int it = 0; it < min(nk, P::STAGES); ++it) load(it, it, true);
         }
     }
     if (warp == 1) {
@@ -400,17 +421,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     before_memory();
 
     if (warp == 0) {
-        if (TMA && elect_one()) {
-            int it = min(nk, P::STAGES);
-            Ring<P::STAGES> r;
-            for (; it < nk; ++it, r.next()) {
-                if (!mbar_wait(empty0 + 8 * r.s, r.phase, &abort)) break;
-                load(it, r.s);
-            }
-            if (abort)                                     // copies in flight land before the CTA ends
-                for (int j = max(it - P::STAGES, 0); j < it; ++j)
-                    mbar_wait(full0 + 8 * (j % P::STAGES), (j / P::STAGES) & 1, nullptr);
-        }
+        if (TMA && elect_one()) produce(min(nk, P::STAGES), true);
     } else if (warp == 1) {
         if (elect_one()) {
             const uint64_t d0 = sw128_desc(base);
@@ -427,7 +438,9 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                          :: "r"(done) : "memory");
         }
-    } else if (!TMA) {                                     // the other warps fill the stages
+    } else if (TMA) {
+        if (warp == 2 && elect_one()) produce(0, false);
+    } else {                                               // the other warps fill the stages
         const int group = (warp - 2) / (LOADERS / 32), lw = (warp - 2) % (LOADERS / 32);
         for (int it = group; it < nk; it += LOAD_GROUPS) {
             const int s = it % P::STAGES;
@@ -454,7 +467,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     bool ok = true;
     __syncwarp();
     if (epi) {
-        ok = warp_wait(done, 0, nullptr);
+        ok = epilogue_wait(done, 0, nullptr, warp == 2, TN == 16 ? 128 : 256);
         ok = __all_sync(~0u, ok && !abort);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
@@ -501,7 +514,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 // would alone take in 48 KB. Persistent: the pair's two accumulators alternate,
 // and a tile's epilogue runs under the next tile's products.
 constexpr int PAIR_EPI_WARPS = 8;
-constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
+constexpr int PAIR_THREADS = 96 + 32 * PAIR_EPI_WARPS;
 constexpr int RASTER = 8;                                  // tiles of tokens walked together
 constexpr int ROW_BYTES = 64;                              // of a token's outputs staged at a time
 
@@ -598,7 +611,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 
     if (tid == 0) {
         for (int i = 0; i < P::STAGES; ++i) {
-            mbar_init(full0 + 8 * i, 1);                   // used in the first CTA only
+            mbar_init(full0 + 8 * i, 2);                   // used in the first CTA only
             mbar_init(empty0 + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -629,9 +642,12 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         n0 = (int)(r / wide) * TN;
     };
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {                          // the tokens' and the channels' copies
         if (elect_one()) {
+            const bool of_x = warp == 0;
+            const uint64_t map = (uint64_t)(of_x ? &map_x : &map_w);
             const uint32_t lead0 = map_to(full0, 0);       // the first CTA's barriers
+            const uint32_t bytes = of_x ? BM * BK : TN / 2 * BK, dst0 = base + (of_x ? 0 : BM * BK);
             Ring<P::STAGES> r;
             uint32_t first = 1;                            // the ring's first round waits for nothing
             bool ok = true;
@@ -639,19 +655,14 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                 int n0;
                 int64_t t0;
                 tile_at(i, t0, n0);
-                const int y0 = (int)t0 + rank * BM, y1 = n0 + rank * (TN / 2);
+                const int y = of_x ? (int)t0 + rank * BM : n0 + rank * (TN / 2);
                 for (int kb = 0; kb < nk; ++kb) {
                     if (!first && !mbar_wait(empty0 + 8 * r.s, r.phase ^ 1u, &abort)) { ok = false; break; }
-                    if (rank == 0) mbar_expect(full0 + 8 * r.s, 2 * P::STAGE);
-                    const uint32_t fb = lead0 + 8 * r.s, dst = base + r.s * P::STAGE;
+                    if (rank == 0) mbar_expect(full0 + 8 * r.s, 2 * bytes);
                     asm volatile(
                         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
                         " [%0], [%1, {%2, %3}], [%4];"
-                        :: "r"(dst), "l"((uint64_t)&map_x), "r"(kb * BK), "r"(y0), "r"(fb) : "memory");
-                    asm volatile(
-                        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-                        " [%0], [%1, {%2, %3}], [%4];"
-                        :: "r"(dst + BM * BK), "l"((uint64_t)&map_w), "r"(kb * BK), "r"(y1), "r"(fb) : "memory");
+                        :: "r"(dst0 + r.s * P::STAGE), "l"(map), "r"(kb * BK), "r"(y), "r"(lead0 + 8 * r.s) : "memory");
                     r.next();
                     if (r.s == 0) first = 0;
                 }
@@ -689,9 +700,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             mbar_wait(drain, 0, nullptr);                  // every MMA issued has completed
         }
     } else {
-        const int q4 = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter, column half
+        const int q4 = warp & 3, half = (warp - 3) >> 2;   // TMEM lane quarter, column half
         constexpr int COLS = TN / 2;
-        uint8_t* mine = smem + P::STAGES * P::STAGE + (warp - 2) * (P::FACTORS + P::STAGED);
+        uint8_t* mine = smem + P::STAGES * P::STAGE + (warp - 3) * (P::FACTORS + P::STAGED);
         float* factors = reinterpret_cast<float*>(mine);
         uint8_t* staged = mine + P::FACTORS;
         Ring<2> acc;
@@ -852,11 +863,11 @@ void pairs(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaSt
               (int)x->dim, (int)mt, (int)nt, e);
 }
 
-// Which kernel, tile and split: the least of the microseconds that these costs, fitted to timings of single launches
-// in a graph, give. A K block of 128 bytes takes 0.195 us in a panel of any width (issue of copies and MMAs) and in a pair
-// 0.20 us with 128 channels, 0.272 us with 256 (the MMAs); the rest is launch, filling the ring and the epilogue. Examples,
-// best panel / pair of 128 / pair of 256: 256 x 1024 x 4096 8.0 / 11.6 / 15.4 us; 512 x 1024 x 1024 6.2 / 6.9 / 8.9;
-// 256 x 4096 x 4096 11.4 / 12.0 / 15.8; 8192 x 4096 x 4096 236 / 112 / 88.
+// Which kernel, tile and split: the least of the microseconds that these costs give, fitted to timings of launches in
+// a graph. A K block of 128 bytes takes 0.14 us in a panel (barriers and issue) and in a pair with 128 channels, 0.272 us
+// in one with 256 (the MMAs), more as all pairs draw on L2; the rest is launch, filling the ring, joining slices and the
+// epilogue. Best panel / pair of 128 / pair of 256, in us: 256 x 1024 x 4096 7.5 / 8.9 / 14.3; 512 x 1024 x 1024
+// 5.2 / 5.5 / 7.8; 256 x 4096 x 4096 10.1 / 9.3 / 14.7; 8192 x 4096 x 4096 236 / 99 / 86.
 struct Plan {
     int tile, split;                                       // split 0: pairs
     double us;
@@ -865,16 +876,19 @@ Plan plan(const jhq_q8_rows* x, const jhq_q8_rows* w) {
     const int64_t nkb = ceil_div(x->dim, BK), mt = ceil_div(w->rows, BM);
     Plan best{256, 0, 0.0};
     for (int tn : {256, 128}) {
-        const double block = tn == 256 ? 0.272 : 0.20, first = tn == 256 ? 6.7 : 5.2, least = tn == 256 ? 6.2 : 3.2;
-        const int64_t waves = ceil_div(ceil_div(x->rows, 2 * BM) * ceil_div(w->rows, tn), SMS / 2);
+        const int64_t tiles = ceil_div(x->rows, 2 * BM) * ceil_div(w->rows, tn), waves = ceil_div(tiles, SMS / 2);
+        const double busy = (double)std::min<int64_t>(tiles, SMS / 2) / (SMS / 2);
+        const double block = tn == 256 ? 0.272 + 0.05 * busy : 0.14 + 0.07 * busy;
+        const double first = tn == 256 ? 5.6 : 4.4, least = tn == 256 ? 4.0 : 2.3;
         const double us = first + nkb * block + (double)(waves - 1) * std::max(nkb * block, least);
         if (tn == 256 || us < best.us) best = {tn, 0, us};
     }
     if (x->rows > 2048) return best;
     for (int tn = 16; tn <= 128; tn *= 2) {
+        const double first = tn == 16 ? 3.0 : tn == 32 ? 3.4 : tn == 64 ? 4.4 : 6.3;
         for (int S = 1; S <= 8 && 2 * S <= std::max<int64_t>(nkb, 2); S *= 2) {
             const int64_t waves = ceil_div(ceil_div(x->rows, tn) * mt * S, panel_capacity(S));
-            const double us = (double)waves * ((double)ceil_div(nkb, S) * 0.195 + (tn == 16 ? 4.0 : tn == 32 ? 4.6 : tn == 64 ? 5.4 : 7.0) + (S > 1 ? 0.8 : 0.0));
+            const double us = (double)waves * ((double)ceil_div(nkb, S) * 0.14 + first + (S > 1 ? 0.9 : 0.0));
             if (us < best.us) best = {tn, S, us};
         }
         if (tn >= x->rows) break;
