@@ -86,11 +86,7 @@ __device__ __forceinline__ void load(const T* p, int left, float* out) {
     if constexpr (A == SINGLE) {
         out[0] = left > 0 ? to_float(*p) : 0.0f;
     } else {
-        if (A == RAGGED && left > 0 && left < V) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = i < left ? to_float(p[i]) : 0.0f;
-            return;
-        }
+        left -= A == RAGGED ? V - 1 : 0;                   // whole pieces alone; mend() follows
         alignas(16) T v[V];
         if constexpr (B >= 16) {
 #pragma unroll
@@ -103,10 +99,19 @@ __device__ __forceinline__ void load(const T* p, int left, float* out) {
         for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
     }
 }
+// The values of a ragged piece, once a thread's whole pieces are on their way.
 template <Access A, int V, class T>
-__device__ __forceinline__ void put(T* p, int left, const float* in) {
+__device__ __forceinline__ void mend(const T* p, int left, float* out) {
+    if (A == RAGGED && left > 0 && left < V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = i < left ? to_float(p[i]) : 0.0f;
+    }
+}
+// odd: p is off its boundary, and the values are stored one by one.
+template <Access A, int V, class T>
+__device__ __forceinline__ void put(T* p, int left, const float* in, bool odd) {
     constexpr int B = V * (int)sizeof(T);
-    if (A == RAGGED && left < V) {
+    if (A != SINGLE && (odd || (A == RAGGED && left < V))) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < left) from_float(p + i, in[i]);
@@ -126,8 +131,8 @@ __device__ __forceinline__ void put(T* p, int left, const float* in) {
     }
 }
 template <Access A, int V>
-__device__ __forceinline__ void put_bytes(int8_t* p, int left, const uint32_t* v) {
-    if (A == RAGGED && left < V) {
+__device__ __forceinline__ void put_bytes(int8_t* p, int left, const uint32_t* v, bool odd) {
+    if (A != SINGLE && (odd || (A == RAGGED && left < V))) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < left) p[i] = (int8_t)v[i];
@@ -204,6 +209,7 @@ struct Args {
     float* scale;
     const int64_t* slots;
     int64_t nslots;
+    bool odd_out, odd_q;                                 // res_out's or q's rows begin off the accesses' boundaries
     unsigned teams;                                      // rows times groups
     int groups, d;                                       // d: values of a group
 };
@@ -239,25 +245,34 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
     const T* x = static_cast<const T*>(a.x) + row * a.ldx + off;
 #pragma unroll
     for (int i = 0; i < NV; ++i) load<A, V, true>(x + at(i), d - at(i), h + i * V);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) mend<A, V>(x + at(i), d - at(i), h + i * V);
     if (NORM && a.res) {
         const R* res = static_cast<const R*>(a.res) + row * a.ldr;
         float r[EPT];
 #pragma unroll
         for (int i = 0; i < NV; ++i) load<A, V, true>(res + at(i), d - at(i), r + i * V);
 #pragma unroll
+        for (int i = 0; i < NV; ++i) mend<A, V>(res + at(i), d - at(i), r + i * V);
+#pragma unroll
         for (int i = 0; i < EPT; ++i) h[i] += r[i];
     }
     if (NORM && a.res_out) {
         R* o = static_cast<R*>(a.res_out) + row * a.ldo;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) put<A, V>(o + at(i), d - at(i), h + i * V);
+        for (int i = 0; i < NV; ++i) put<A, V>(o + at(i), d - at(i), h + i * V, a.odd_out);
     }
     auto weigh = [&](float* w, int i) {                    // the weights of piece i
         if (!NORM || !a.weight) {
 #pragma unroll
             for (int j = 0; j < V; ++j) w[j] = 1.0f;
-        } else if (a.w32) load<A, V, false>(static_cast<const float*>(a.weight) + at(i), d - at(i), w);
-        else load<A, V, false>(static_cast<const T*>(a.weight) + at(i), d - at(i), w);
+        } else if (a.w32) {
+            load<A, V, false>(static_cast<const float*>(a.weight) + at(i), d - at(i), w);
+            mend<A, V>(static_cast<const float*>(a.weight) + at(i), d - at(i), w);
+        } else {
+            load<A, V, false>(static_cast<const T*>(a.weight) + at(i), d - at(i), w);
+            mend<A, V>(static_cast<const T*>(a.weight) + at(i), d - at(i), w);
+        }
     };
     float sum = 0.0f, top = 0.0f;
     auto gather = [&](float by) {
@@ -303,7 +318,7 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
             uint32_t b[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) b[j] = quant.plain(NORM ? h[i * V + j] * w[j] : h[i * V + j]);
-            put_bytes<A, V>(q + at(i), keep - at(i), b);
+            put_bytes<A, V>(q + at(i), keep - at(i), b, a.odd_q);
         }
     } else {
 #pragma unroll
@@ -313,7 +328,7 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
             uint32_t b[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) b[j] = quant(NORM ? h[i * V + j] * by * w[j] : h[i * V + j]);
-            put_bytes<A, V>(q + at(i), keep - at(i), b);
+            put_bytes<A, V>(q + at(i), keep - at(i), b, a.odd_q);
         }
     }
     if (me == 0 && wanted) {
@@ -404,19 +419,26 @@ void launch_rows(const Args& a, cudaStream_t s) {
     const bool few = a.teams <= 2 * SMS && d > 256;
     if (!NORM && d <= 16) return launch_team<T, R, 2, 8, A, NORM>(a, s);
     if (!NORM && d <= 32) return launch_team<T, R, 4, 8, A, NORM>(a, s);
-    if (!NORM && d <= 64) return launch_team<T, R, 4, 16, A, NORM>(a, s);
-    if (d <= 128) return launch_team<T, R, 8, 16, A, NORM>(a, s);
-    if (d <= 256) return launch_team<T, R, 16, 16, A, NORM>(a, s);
     if (few && d <= 8 * MOST_THREADS) return launch_block<T, R, 8, A, NORM>(a, s);
     if (few && d <= 16 * MOST_THREADS) return launch_block<T, R, 16, A, NORM>(a, s);
-    if (d <= 512) return launch_team<T, R, 32, 16, A, NORM>(a, s);
     if constexpr (A == SINGLE) {
+        if (!NORM && d <= 64) return launch_team<T, R, 4, 16, A, NORM>(a, s);
+        if (d <= 128) return launch_team<T, R, 8, 16, A, NORM>(a, s);
+        if (d <= 256) return launch_team<T, R, 16, 16, A, NORM>(a, s);
+        if (d <= 512) return launch_team<T, R, 32, 16, A, NORM>(a, s);
         if (d <= 1024) return launch_team<T, R, 64, 16, A, NORM>(a, s);
         if (d <= 2048) return launch_team<T, R, 128, 16, A, NORM>(a, s);
         if (d <= 4096) return launch_team<T, R, 256, 16, A, NORM>(a, s);
         if (d <= 8192) return launch_team<T, R, 512, 16, A, NORM>(a, s);
     } else {
+        if (!NORM && d <= 64) return launch_team<T, R, 2, 32, A, NORM>(a, s);
+        if (d <= 128) return launch_team<T, R, 4, 32, A, NORM>(a, s);
+        if (d <= 256) return launch_team<T, R, 8, 32, A, NORM>(a, s);
+        if (d <= 512) return launch_team<T, R, 16, 32, A, NORM>(a, s);
         if (d <= 1024) return launch_team<T, R, 32, 32, A, NORM>(a, s);
+        // float32 rows and residuals, 128 bytes of each a thread, leave too few threads room
+        // (16384 x 2560: 95 us with 32 values, 86 us with 16)
+        if (NORM && sizeof(T) == 4 && a.res && d <= 16 * MOST_THREADS) return launch_block<T, R, 16, A, NORM>(a, s);
         if (d <= 32 * MOST_THREADS) return launch_block<T, R, 32, A, NORM>(a, s);
     }
     launch_q8(long_rows_kernel<T, R, NORM>, dim3(a.teams), LONG_THREADS, 0, 0, s, a);
@@ -658,9 +680,10 @@ void q8_rms_norm(const jhq_view* x, const jhq_view* residual, const jhq_view* we
         auto go = [&](auto r) {
             using R = decltype(r);
             const int rb = std::min(16, V * (int)sizeof(R));
-            const bool vec = on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) && on_bytes(a.q, a.ldq, 1, V, x->rows) &&
-                             on_bytes(a.res, a.ldr, sizeof(R), rb, x->rows) &&
-                             on_bytes(a.res_out, a.ldo, sizeof(R), rb, x->rows) && (uintptr_t)a.weight % 16 == 0;
+            const bool vec = on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) && on_bytes(a.res, a.ldr, sizeof(R), rb, x->rows) &&
+                             (uintptr_t)a.weight % 16 == 0;
+            a.odd_q = !on_bytes(a.q, a.ldq, 1, V, x->rows);
+            a.odd_out = !on_bytes(a.res_out, a.ldo, sizeof(R), rb, x->rows);
             if (!vec) launch_rows<T, R, SINGLE, true>(a, s);
             else if (a.d % V == 0) launch_rows<T, R, WHOLE, true>(a, s);
             else launch_rows<T, R, RAGGED, true>(a, s);
