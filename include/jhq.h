@@ -317,7 +317,7 @@ int jhq_q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* 
 
 /* After the streams of the calls above have drained: JHQ_ETIMEDOUT (once) if a
  * bounded device wait of one of them on the current device gave up, so that its
- * output is not valid, else JHQ_OK. Synchronises with the device. */
+ * output is not valid, else JHQ_OK. */
 int jhq_q8_status(void);
 
 /* ---- per-stage timing (the reference's jhq_v9_step_timing / v13 step

@@ -7,8 +7,8 @@
 //
 // Every wait on an mbarrier is bounded (about a second); one that gives up sets
 // g_q8_error (jhq_q8_status) and the CTA's abort flag, which ends every role's
-// loop. Before it leaves, a CTA lets the copies and MMAs it issued finish (bounded
-// again) and frees its TMEM.
+// loop. Before it leaves, a CTA lets the MMAs (bounded again) and the copies (for a
+// fixed time) that it issued finish and frees its TMEM.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 #include <mutex>
 
 #include "kernels.cuh"
@@ -35,6 +36,7 @@ struct Epilogue {                   // what turns a sum into an output
     int64_t T;
     int N, type;
     bool vec;                       // output rows begin on 16-byte boundaries
+    long long limit;                // cycles that a wait may take
 };
 
 __device__ __forceinline__ void store(float* p, float v) { *p = v; }
@@ -63,19 +65,34 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 
 // Bounded wait for the phase of parity `parity`; gives up when the CTA's abort
-// flag is set or after WAIT_CYCLES, which sets the flag and g_q8_error.
-__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-    if (mbar_try(bar, parity)) return true;
+// flag is set or after `limit` cycles (at once if 0), which sets the flag and
+// g_q8_error. The waits of a launch use its limit (WAIT_CYCLES unless a test shortens
+// it); those for what was issued before an abort have abort = nullptr and WAIT_CYCLES.
+__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit = WAIT_CYCLES) {
+    if (limit > 0 && mbar_try(bar, parity)) return true;
     const long long t0 = clock64();
-    while (!mbar_try(bar, parity)) {
+    do {
         if (abort && *abort) return false;
-        if (clock64() - t0 > WAIT_CYCLES) {
+        if (clock64() - t0 >= limit) {
             atomicExch(&g_q8_error, 1);
             if (abort) *abort = 1;
             return false;
         }
-    }
+    } while (!mbar_try(bar, parity));
     return true;
+}
+// Before a CTA ends (all threads call it, their roles done): after an abort copies
+// may still be in flight, whose barriers no longer tell; they land within microseconds
+// and are given 2^24 cycles (8 ms).
+__device__ __forceinline__ void settle(volatile int* abort) {
+    __syncthreads();
+    if (*abort) {
+        if (threadIdx.x == 0) {
+            const long long t0 = clock64();
+            while (clock64() - t0 < (1ll << 24)) {}
+        }
+        __syncthreads();
+    }
 }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -197,17 +214,17 @@ __device__ __forceinline__ void get_scales(const Epilogue& e, int64_t t, float* 
     }
 }
 // A warp's wait: lane 0 polls.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
     bool ok = true;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort);
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort, limit);
     return __all_sync(~0u, ok);
 }
 // The wait of a panel's epilogue warps, through the whole of its products: the first
 // one's lane 0 polls, the others sleep at a barrier. (With all eight polling, the barrier
 // operations of the producers and the MMA thread took 0.16 us a K block.)
-__device__ __forceinline__ bool epilogue_wait(uint32_t bar, uint32_t parity, volatile int* abort, bool polls, int threads) {
+__device__ __forceinline__ bool epilogue_wait(uint32_t bar, uint32_t parity, bool polls, int threads) {
     bool ok = true;
-    if (polls && (threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort);
+    if (polls && (threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, nullptr);
     __syncwarp();
     uint32_t all;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
@@ -384,12 +401,9 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         const uint32_t odd = it == 0 ? 1u : 0u;            // the ring's second round waits for the first phase
         Ring<P::STAGES> r;                                 // begins at a multiple of STAGES, or ends there
         for (; it < nk; ++it, r.next()) {
-            if (it >= P::STAGES && !mbar_wait(empty0 + 8 * r.s, r.phase ^ odd, &abort)) break;
+            if (it >= P::STAGES && !mbar_wait(empty0 + 8 * r.s, r.phase ^ odd, &abort, e.limit)) break;
             load(it, r.s, of_w);
         }
-        if (abort)                                         // copies in flight land before the CTA ends
-            for (int j = max(it - P::STAGES, 0); j < it; ++j)
-                mbar_wait(full0 + 8 * (j % P::STAGES), (j / P::STAGES) & 1, nullptr);
     };
 
     if (tid == 0) {
@@ -428,7 +442,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             int left = K - kb0 * BK;
             Ring<P::STAGES> r;
             for (int it = 0; it < nk; ++it, r.next(), left -= BK) {
-                if (!mbar_wait(full0 + 8 * r.s, r.phase, &abort)) break;
+                if (!mbar_wait(full0 + 8 * r.s, r.phase, &abort, e.limit)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t d = d0 + (uint64_t)(r.s * (P::STAGE >> 4));
                 mma_block<1>(tmem, d, d + (BM * BK >> 4), idesc_i8(BM, TN), left, it > 0);
@@ -444,7 +458,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         const int group = (warp - 2) / (LOADERS / 32), lw = (warp - 2) % (LOADERS / 32);
         for (int it = group; it < nk; it += LOAD_GROUPS) {
             const int s = it % P::STAGES;
-            if (it >= P::STAGES && !warp_wait(empty0 + 8 * s, (it / P::STAGES - 1) & 1, &abort)) break;
+            if (it >= P::STAGES && !warp_wait(empty0 + 8 * s, (it / P::STAGES - 1) & 1, &abort, e.limit)) break;
             const uint32_t dst = base + s * P::STAGE;
             const int k = (kb0 + it) * BK;
             load_stage<TN>(w, x, m0, t0, k, K, dst, lw, lane);
@@ -467,7 +481,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     bool ok = true;
     __syncwarp();
     if (epi) {
-        ok = epilogue_wait(done, 0, nullptr, warp == 2, TN == 16 ? 128 : 256);
+        ok = epilogue_wait(done, 0, warp == 2, TN == 16 ? 128 : 256);
         ok = __all_sync(~0u, ok && !abort);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
@@ -501,7 +515,7 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         cluster_sync();                                    // no CTA leaves while its sums are read
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    settle(&abort);
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(P::COLS));
 }
@@ -657,7 +671,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                 tile_at(i, t0, n0);
                 const int y = of_x ? (int)t0 + rank * BM : n0 + rank * (TN / 2);
                 for (int kb = 0; kb < nk; ++kb) {
-                    if (!first && !mbar_wait(empty0 + 8 * r.s, r.phase ^ 1u, &abort)) { ok = false; break; }
+                    if (!first && !mbar_wait(empty0 + 8 * r.s, r.phase ^ 1u, &abort, e.limit)) { ok = false; break; }
                     if (rank == 0) mbar_expect(full0 + 8 * r.s, 2 * bytes);
                     asm volatile(
                         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -667,10 +681,6 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                     if (r.s == 0) first = 0;
                 }
             }
-            if (!ok) {                                     // copies in flight land before the CTA ends: the
-                const long long c0 = clock64();            // second CTA cannot wait on the first's barriers
-                while (clock64() - c0 < (1ll << 24)) {}
-            }
         }
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
@@ -679,11 +689,11 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             Ring<2> acc;
             bool ok = true;
             for (int64_t i = pair; ok && i < tiles; i += npairs, acc.next()) {
-                if (i >= pair + 2 * (int64_t)npairs && !mbar_wait(tempty0 + 8 * acc.s, acc.phase ^ 1u, &abort)) break;
+                if (i >= pair + 2 * (int64_t)npairs && !mbar_wait(tempty0 + 8 * acc.s, acc.phase ^ 1u, &abort, e.limit)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 int left = K;
                 for (int kb = 0; kb < nk; ++kb, r.next(), left -= BK) {
-                    if (!mbar_wait(full0 + 8 * r.s, r.phase, &abort)) { ok = false; break; }
+                    if (!mbar_wait(full0 + 8 * r.s, r.phase, &abort, e.limit)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t d = d0 + (uint64_t)(r.s * (P::STAGE >> 4));
                     mma_block<2>(tmem + acc.s * TN, d, d + (BM * BK >> 4), idesc_i8(2 * BM, TN), left, kb > 0);
@@ -736,7 +746,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             }
             __syncwarp();
             fetch(i + npairs);                             // arrives under this tile's products and outputs
-            if (!warp_wait(tfull0 + 8 * acc.s, acc.phase, &abort)) break;
+            if (!warp_wait(tfull0 + 8 * acc.s, acc.phase, &abort, e.limit)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem + ((uint32_t)(q4 * 32) << 16) + acc.s * TN + half * COLS;
             if (t1 < e.T) {
@@ -755,7 +765,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    settle(&abort);
     cluster_sync();                                        // no MMA or arrival still heads for the other CTA
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t)(2 * TN)));
@@ -922,9 +932,11 @@ void q8_matmul(const jhq_q8_rows* x, const jhq_q8_rows* w, const jhq_view* bias,
         if (bias->type != JHQ_F32 || bias->rows != 1 || bias->cols != out->cols)
             fail(JHQ_EINVAL, "q8_matmul: bias must be 1 x w's rows of float32");
     }
+    long long limit = WAIT_CYCLES;
+    if (const char* v = std::getenv("JHQ_TEST_TC_WAIT_CYCLES")) limit = std::atoll(v);
     const Epilogue e{x->scale, w->scale, bias ? (const float*)bias->data : nullptr, out->data, out->ld,
                      x->rows, (int)w->rows, out->type,
-                     (uintptr_t)out->data % 16 == 0 && out->ld % (out->type == JHQ_F32 ? 4 : 8) == 0};
+                     (uintptr_t)out->data % 16 == 0 && out->ld % (out->type == JHQ_F32 ? 4 : 8) == 0, limit};
     const bool tma = on_boundaries(x) && on_boundaries(w);
     const Plan p = tma ? plan(x, w) : plan_unaligned(x, w);
     if (!tma) panels<false>(x, w, p.tile, p.split, e, s);

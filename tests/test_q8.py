@@ -436,6 +436,26 @@ def test_calls_wait_for_one_another(jhq, t, d, n):
 
 
 @gpu
+@pytest.mark.parametrize("t,n,k,packed", [(1, 1024, 8192, False), (100, 300, 4096, False), (40, 300, 999, True),
+                                          (700, 900, 640, False), (5000, 2000, 2048, False)])
+def test_waits_that_give_up_are_reported(jhq, monkeypatch, t, n, k, packed):
+    """With no cycles to wait (JHQ_TEST_TC_WAIT_CYCLES, read at the launch) every wait gives up: the kernel ends by
+    itself, the status says so once, and the next call is whole again."""
+    monkeypatch.setenv("JHQ_TEST_TC_WAIT_CYCLES", "0")
+    qx, sx = _q8(95, t, k, k if packed else None)
+    qw, sw = _q8(96, n, k, k if packed else None)
+    out = torch.zeros(t, n, device="cuda")
+    jhq.q8_matmul(jhq.Q8Rows.of(qx, sx), jhq.Q8Rows.of(qw, sw), jhq.View.of(out), stream=_stream())
+    torch.cuda.synchronize()
+    with pytest.raises(jhq.JHQError) as e:
+        jhq.q8_check_status()
+    assert e.value.code == jhq.JHQ_ETIMEDOUT
+    jhq.q8_check_status()
+    monkeypatch.delenv("JHQ_TEST_TC_WAIT_CYCLES")
+    _mm_check(jhq, t, n, k, torch.float32, False)
+
+
+@gpu
 def test_launches_are_counted(jhq):
     x = _randn(91, 4, 64)
     q, s = torch.empty(4, 64, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
