@@ -56,10 +56,31 @@ __device__ __forceinline__ void from_float(float* p, float v) { *p = v; }
 __device__ __forceinline__ void from_float(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ void pack2(uint32_t* p, float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    *p = *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void pack2(uint32_t* p, float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    *p = *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two 16-bit values of a word, as floats.
+__device__ __forceinline__ void unpack2(uint32_t w, float* out, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    out[0] = f.x;
+    out[1] = f.y;
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float* out, __nv_bfloat16) {
+    out[0] = __uint_as_float(w << 16);
+    out[1] = __uint_as_float(w & 0xffff0000u);
+}
+
 // How a thread touches its piece of V values at p, of which the first `left` are
 // the row's: single values (V = 1), whole pieces of 16 bytes of x (all or nothing
-// is the row's), or whole pieces with a ragged last one, value by value.
-enum Access { SINGLE, WHOLE, RAGGED };
+// is the row's), the same with a ragged last one, value by value, or whole pieces
+// that are all there.
+enum Access { SINGLE, WHOLE, RAGGED, FULL };
 
 __device__ __forceinline__ uint4 load16(const void* p) {     // not kept in L1, which is left to the weights
     uint4 v;
@@ -87,16 +108,28 @@ __device__ __forceinline__ void load(const T* p, int left, float* out) {
         out[0] = left > 0 ? to_float(*p) : 0.0f;
     } else {
         left -= A == RAGGED ? V - 1 : 0;                   // whole pieces alone; mend() follows
-        alignas(16) T v[V];
+        uint32_t v[B / 4];
         if constexpr (B >= 16) {
 #pragma unroll
-            for (int i = 0; i < B / 16; ++i) load_if<STREAM>(left > 0, reinterpret_cast<const uint4*>(p) + i, reinterpret_cast<uint4*>(v)[i]);
+            for (int i = 0; i < B / 16; ++i) {
+                const uint4* from = reinterpret_cast<const uint4*>(p) + i;
+                uint4 u;
+                if constexpr (A != FULL) load_if<STREAM>(left > 0, from, u);
+                else u = STREAM ? load16(from) : *from;
+                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+            }
         } else {
             static_assert(B == 8, "four 16-bit weights or residuals of float32 rows");
-            *reinterpret_cast<uint2*>(v) = left > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+            const uint2 u = A == FULL || left > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+            v[0] = u.x; v[1] = u.y;
         }
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = to_float(v[i]);
+            for (int i = 0; i < V; i += 2) unpack2(v[i / 2], out + i, T());
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[i] = __uint_as_float(v[i]);
+        }
     }
 }
 // The values of a ragged piece, once a thread's whole pieces are on their way.
@@ -119,8 +152,13 @@ __device__ __forceinline__ void put(T* p, int left, const float* in, bool odd) {
     }
     if (left <= 0) return;
     alignas(16) T v[V];
+    if constexpr (sizeof(T) == 2 && V > 1) {               // two at a time
 #pragma unroll
-    for (int i = 0; i < V; ++i) from_float(&v[i], in[i]);
+        for (int i = 0; i < V; i += 2) pack2(reinterpret_cast<uint32_t*>(v) + i / 2, in[i], in[i + 1], T());
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) from_float(&v[i], in[i]);
+    }
     if constexpr (B >= 16) {
 #pragma unroll
         for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
@@ -165,9 +203,9 @@ struct Quant {
     __device__ uint32_t plain(float g) const { return __float_as_uint(g * inv + 12582912.0f); }   // fine, pre = 1
     __device__ uint32_t operator()(float g) const { return fine ? plain(g * pre) : 0u; }
 };
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {   // of a and |b|; NaN if either is
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // Sum and maximum over a team: up to 32 lanes of a warp, or the block (of TEAM
@@ -219,14 +257,18 @@ constexpr int SMS = 148;
 // holds EPT values each in registers, so x and the residual are read once and
 // every output is written once. Bound by those bytes, as long as a thread has
 // enough values that the instructions spent on a row and not on a value (addresses,
-// the team's reductions, the reciprocal) stay few. Short groups share a warp, rows
-// to 1024 values have a warp, longer ones a block, of as many threads as they need
-// (TEAM = 0) or, for single values, whose addresses then differ by constants, of TEAM
-// (20000 x 1001 in bfloat16, packed: 100 instructions a value without that). Registers are held to
-// what lets an SM hold 768 threads with 32 values each, 1024 with fewer.
+// the team's reductions, the reciprocal) stay few: 27 a value in all for a norm. Short
+// groups share a warp, rows to 1024 values have a warp, longer ones a block, of as many
+// threads as they need (TEAM = 0) or, for single values, of TEAM, so that their
+// addresses differ by constants (20000 x 1001 in bfloat16, packed: 84 us without, 60 us
+// with). Registers are held to 64, and to 80 where a thread holds 32 float32 values or
+// residuals.
+// Measured: norm of 65536 x 4096 in bfloat16 with its residual 299 us (6.28 TB/s, 0.96 of
+// a copy's rate), with a float32 residual 476 us (6.20 TB/s); 1 x 4096 2.6 us; 65536 x 1024
+// 78 us (6.02 TB/s); cache write of 65536 x 16 x 128 in bfloat16 71 us (5.65 TB/s).
 constexpr int SHARED_BLOCK = 128, MOST_THREADS = 512;
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
-__global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_constant__ Args a) {
+__global__ void __maxnreg__(EPT == 32 && (sizeof(T) == 4 || sizeof(R) == 4) ? 80 : 64) rows_kernel(const __grid_constant__ Args a) {
     constexpr int V = A == SINGLE ? 1 : 16 / (int)sizeof(T), NV = EPT / V;
     let_next_start();
     before_memory();
@@ -285,7 +327,7 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
             for (int j = 0; j < V; ++j) {
                 const float v = h[i * V + j] * by;
                 if (NORM) sum = __fmaf_rn(v, v, sum);
-                top = max_nan(top, fabsf(v * w[j]));
+                top = max_nan(top, v * w[j]);
             }
         }
     };
@@ -298,7 +340,7 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
         // near the ends of float32's range: again with h scaled by a power of two
         float hm = 0.0f;
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) hm = max_nan(hm, fabsf(h[i]));
+        for (int i = 0; i < EPT; ++i) hm = max_nan(hm, h[i]);
         const float htop = team_sum_max<TEAM>(0.0f, hm, red[1]).y;
         if (odd && htop > 0.0f && is_finite(htop)) by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
         gather(by);
@@ -340,7 +382,8 @@ __global__ void __maxnreg__(EPT == 32 ? 80 : 64) rows_kernel(const __grid_consta
 }
 
 // Rows longer than a block's registers: the row is read twice (thrice near the
-// ends of float32's range).
+// ends of float32's range), value by value: bound by instructions. Measured: norm of 4096 x
+// 32768 in bfloat16 335 us (2.8 TB/s).
 constexpr int LONG_THREADS = 1024;
 template <class T, class R, bool NORM>
 __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_constant__ Args a) {
@@ -369,7 +412,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
         for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) {
             const float h = h_of(j) * by;
             if (NORM) sum = __fmaf_rn(h, h, sum);
-            top = max_nan(top, fabsf(h * w_of(j)));
+            top = max_nan(top, h * w_of(j));
         }
         return team_sum_max<0>(sum, top, r);
     };
@@ -379,7 +422,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
         step = top_g / (127.0f * sqrtf(st.x / (float)a.d + a.eps));
         if (!(st.x >= 0x1p-90f && st.x <= 0x1p120f && top_g >= 0x1p-100f && top_g <= 0x1p120f)) {
             float hm = 0.0f;
-            for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max_nan(hm, fabsf(h_of(j)));
+            for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max_nan(hm, h_of(j));
             const float htop = team_sum_max<0>(0.0f, hm, red[1]).y;
             if (htop > 0.0f && is_finite(htop)) {
                 by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
@@ -402,11 +445,15 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
 
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 void launch_team(const Args& a, cudaStream_t s) {
+    if constexpr (A == WHOLE)
+        if (a.d == TEAM * EPT) return launch_team<T, R, TEAM, EPT, FULL, NORM>(a, s);
     constexpr unsigned per = TEAM <= 32 ? SHARED_BLOCK / TEAM : 1;
     launch_q8(rows_kernel<T, R, TEAM, EPT, A, NORM>, dim3((a.teams - 1) / per + 1), TEAM <= 32 ? SHARED_BLOCK : TEAM, 0, 0, s, a);
 }
 template <class T, class R, int EPT, Access A, bool NORM>
 void launch_block(const Args& a, cudaStream_t s) {
+    if constexpr (A == WHOLE)
+        if (a.d % (32 * EPT) == 0) return launch_block<T, R, EPT, FULL, NORM>(a, s);
     launch_q8(rows_kernel<T, R, 0, EPT, A, NORM>, dim3(a.teams), (a.d - 1) / EPT / 32 * 32 + 32, 0, 0, s, a);
 }
 // Many rows: the smallest team whose registers hold a row at 32 values a thread (at 16 and 8 the instructions spent on
@@ -449,7 +496,9 @@ bool on_bytes(const void* p, int64_t ld, int size, int rows_of, int64_t rows) {
 }
 
 // Reads rows back: V values of a row a thread (32 bytes of output where rows
-// allow it), TPR threads a row. Bound by the bytes: one in, sizeof(T) out a value.
+// allow it: 16 took 125 us for the case below), tpr threads a row, several rows a thread
+// when there are many. Bound by the bytes: one in, sizeof(T) out a value. Measured: 65536 x
+// 2048 bfloat16 values from rows in any order 69 us (5.80 TB/s).
 template <class T, int V>
 struct alignas(V * sizeof(T)) Piece {
     T v[V];
@@ -539,6 +588,8 @@ __device__ __noinline__ uint32_t word_edge(const int8_t* p, const int8_t* first,
 // Rows at odd addresses or of odd groups: a thread takes the V values of an aligned
 // 32 bytes of output (the first and last piece of a row: of what the row has of
 // them) and gathers their bytes from aligned words. WALK: groups shorter than a piece.
+// Measured: 30000 x 7 x 333 bfloat16 values 97 us (2.15 TB/s; 238 us value by value),
+// bound by instructions.
 template <class T, bool WALK>
 __global__ void __launch_bounds__(256)
 read_odd_kernel(const int8_t* __restrict__ q, int64_t ldq, const int8_t* __restrict__ end, const float* __restrict__ scale,
