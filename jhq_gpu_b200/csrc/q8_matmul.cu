@@ -243,7 +243,7 @@ __device__ __forceinline__ bool epilogue_wait(uint32_t bar, uint32_t parity, boo
 // Bound by the weights' bytes for long rows, by launch, ring and epilogue (3 to 5 us) for
 // short ones. Measured: 1 x 8192 x 8192 13.7 us (4.9 TB/s, 0.75 of a copy's rate), 64 x 8192
 // x 8192 16.2 us (4.2 TB/s), 1 x 1024 x 4096 3.8 us, 256 x 1024 x 4096 7.6 us; from rows at
-// odd addresses, bound by the loads' latency, 1000 x 999 x 1001 14.6 us, 4001 x 4001 x 4001
+// odd addresses, bound by the loads' latency, 1000 x 999 x 1001 14.0 us, 4001 x 4001 x 4001
 // 408 us (314 TOP/s).
 constexpr int BM = 128, BK = 128;
 constexpr int LOADERS = 256;                               // threads of the epilogue, which load where TMA cannot
@@ -894,8 +894,21 @@ struct Plan {
     int tile, split;                                       // split 0: pairs
     double us;
 };
-Plan plan(const jhq_q8_rows* x, const jhq_q8_rows* w) {
+// The best panel, if it beats `best`: tiles of 16, 32, 64 and 128 tokens at block[] us a K block and first[] us a tile.
+void best_panel(const jhq_q8_rows* x, const jhq_q8_rows* w, const double* block, const double* first, Plan& best) {
     const int64_t nkb = ceil_div(x->dim, BK), mt = ceil_div(w->rows, BM);
+    for (int k = 0; k < 4; ++k) {
+        const int tn = 16 << k;
+        for (int S = 1; S <= 8 && 2 * S <= std::max<int64_t>(nkb, 2); S *= 2) {
+            const int64_t waves = ceil_div(ceil_div(x->rows, tn) * mt * S, panel_capacity(S));
+            const double us = (double)waves * ((double)ceil_div(nkb, S) * block[k] + first[k] + (S > 1 ? 0.9 : 0.0));
+            if (us < best.us) best = {tn, S, us};
+        }
+        if (tn >= x->rows) break;
+    }
+}
+Plan plan(const jhq_q8_rows* x, const jhq_q8_rows* w) {
+    const int64_t nkb = ceil_div(x->dim, BK);
     Plan best{256, 0, 0.0};
     for (int tn : {256, 128}) {
         const int64_t tiles = ceil_div(x->rows, 2 * BM) * ceil_div(w->rows, tn), waves = ceil_div(tiles, SMS / 2);
@@ -906,23 +919,18 @@ Plan plan(const jhq_q8_rows* x, const jhq_q8_rows* w) {
         if (tn == 256 || us < best.us) best = {tn, 0, us};
     }
     if (x->rows > 2048) return best;
-    for (int tn = 16; tn <= 128; tn *= 2) {
-        const double first = tn == 16 ? 3.0 : tn == 32 ? 3.4 : tn == 64 ? 4.4 : 6.3;
-        for (int S = 1; S <= 8 && 2 * S <= std::max<int64_t>(nkb, 2); S *= 2) {
-            const int64_t waves = ceil_div(ceil_div(x->rows, tn) * mt * S, panel_capacity(S));
-            const double us = (double)waves * ((double)ceil_div(nkb, S) * 0.14 + first + (S > 1 ? 0.9 : 0.0));
-            if (us < best.us) best = {tn, S, us};
-        }
-        if (tn >= x->rows) break;
-    }
+    const double block[4] = {0.14, 0.14, 0.14, 0.14}, first[4] = {3.0, 3.4, 4.4, 6.3};
+    best_panel(x, w, block, first, best);
     return best;
 }
-// Rows that TMA cannot fetch: the loader threads bind, who bring 128 + tile rows for 128 x tile products.
+// Rows that TMA cannot fetch: panels, whose loader threads bind, who bring 128 + tile rows for 128 x tile products.
+// 1 x 4001 x 4001 in tiles of 16 took 32 / 18 / 11.5 us in 1 / 2 / 4 slices, 1000 x 999 x 1001 in tiles of 64 14.0 us, of
+// 128 in two slices 15.4 us, 4001 x 4001 x 4001 in tiles of 64 555 us, of 128 428 us.
 Plan plan_unaligned(const jhq_q8_rows* x, const jhq_q8_rows* w) {
-    Plan p{x->rows <= 16 ? 16 : x->rows <= 32 ? 32 : x->rows <= 64 ? 64 : 128, 1, 0.0};
-    const int64_t tiles = ceil_div(x->rows, p.tile) * ceil_div(w->rows, BM), nkb = ceil_div(x->dim, BK);
-    while (p.split < 8 && nkb >= 4 * p.split && tiles * p.split * 2 <= panel_capacity(2 * p.split)) p.split *= 2;
-    return p;
+    Plan best{128, 1, 1e30};
+    const double block[4] = {0.85, 0.85, 1.0, 1.5}, first[4] = {4.8, 5.0, 5.4, 6.5};
+    best_panel(x, w, block, first, best);
+    return best;
 }
 
 }  // namespace
