@@ -458,16 +458,17 @@ void launch_block(const Args& a, cudaStream_t s) {
 }
 // Many rows: the smallest team whose registers hold a row at 32 values a thread (at 16 and 8 the instructions spent on
 // a row bind: 65536 x 4096 in bfloat16 took 441 us with 16, 303 us with 32), at 16 single values, whose registers
-// 32 do not fit. Few rows, which leave SMs idle: as few values a thread as a block allows (1 x 4096: 3.4 us with 16,
-// 3.8 us with 32).
+// 32 do not fit. Few rows: 8 or 16 values a thread where all rows then run at once (1 x 4096: 2.6 us with 8, 3.8 us with
+// 32; 2000 x 1024: 4.5 us with 16, 5.7 us with 32; but 4000 x 1024: 8.3 and 6.9 us).
 template <class T, class R, Access A, bool NORM>
 void launch_rows(const Args& a, cudaStream_t s) {
     const int d = a.d;
-    const bool few = a.teams <= 2 * SMS && d > 256;
+    // whether all rows, `each` values a thread, are on the SMs at once
+    const auto fits = [&](int each) { return d > 256 && d <= each * MOST_THREADS && (int64_t)a.teams * ((d - 1) / each + 1) <= SMS * 1024; };
     if (!NORM && d <= 16) return launch_team<T, R, 2, 8, A, NORM>(a, s);
     if (!NORM && d <= 32) return launch_team<T, R, 4, 8, A, NORM>(a, s);
-    if (few && d <= 8 * MOST_THREADS) return launch_block<T, R, 8, A, NORM>(a, s);
-    if (few && d <= 16 * MOST_THREADS) return launch_block<T, R, 16, A, NORM>(a, s);
+    if (fits(8)) return launch_block<T, R, 8, A, NORM>(a, s);
+    if (fits(16)) return launch_block<T, R, 16, A, NORM>(a, s);
     if constexpr (A == SINGLE) {
         if (!NORM && d <= 64) return launch_team<T, R, 4, 16, A, NORM>(a, s);
         if (d <= 128) return launch_team<T, R, 8, 16, A, NORM>(a, s);
@@ -482,10 +483,11 @@ void launch_rows(const Args& a, cudaStream_t s) {
         if (d <= 128) return launch_team<T, R, 4, 32, A, NORM>(a, s);
         if (d <= 256) return launch_team<T, R, 8, 32, A, NORM>(a, s);
         if (d <= 512) return launch_team<T, R, 16, 32, A, NORM>(a, s);
-        if (d <= 1024) return launch_team<T, R, 32, 32, A, NORM>(a, s);
+        const bool wide = NORM && sizeof(T) == 4 && a.res;
+        if (d <= 1024 && !wide) return launch_team<T, R, 32, 32, A, NORM>(a, s);
         // float32 rows and residuals, 128 bytes of each a thread, leave too few threads room
-        // (16384 x 2560: 95 us with 32 values, 86 us with 16)
-        if (NORM && sizeof(T) == 4 && a.res && d <= 16 * MOST_THREADS) return launch_block<T, R, 16, A, NORM>(a, s);
+        // (16384 x 2560: 95 us with 32 values, 86 us with 16; 4099 x 1024: 14.1 and 11.3 us)
+        if (wide && d <= 16 * MOST_THREADS) return launch_block<T, R, 16, A, NORM>(a, s);
         if (d <= 32 * MOST_THREADS) return launch_block<T, R, 32, A, NORM>(a, s);
     }
     launch_q8(long_rows_kernel<T, R, NORM>, dim3(a.teams), LONG_THREADS, 0, 0, s, a);
