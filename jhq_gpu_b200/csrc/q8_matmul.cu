@@ -535,8 +535,8 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 // and a tile's epilogue runs under the next tile's products. Tokens are the rows
 // here so that a thread has neighbouring outputs of one token (5 instructions an
 // output; 32 with channels as rows and 2-byte stores). Bound by the tensor cores, and
-// over seconds by the power limit. Measured: 32768 x 8192 x 8192 1280 us in a burst (3.44
-// POP/s; twice the bfloat16 rate of a library product is 3.32), 1540 us sustained (2.86;
+// over seconds by the power limit. Measured: 32768 x 8192 x 8192 1270 us in a burst (3.46
+// POP/s; twice the bfloat16 rate of a library product is 3.32), 1556 us sustained (2.83;
 // twice its sustained rate is 2.77); 8192 x 4096 x 4096 87 us (3.14, tensor pipe 89%
 // active); 65536 x 1024 x 4096 184 us; 65536 x 512 x 512, bound by outputs, 30 us.
 constexpr int PAIR_EPI_WARPS = 8;
@@ -646,7 +646,6 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
         mbar_init(drain, 1);
         abort = 0;
-        let_next_start();
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -693,6 +692,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                     if (r.s == 0) first = 0;
                 }
             }
+            if (of_x) let_next_start();                    // under the last tile: called at the start, it cost a norm that followed 40 us
         }
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
