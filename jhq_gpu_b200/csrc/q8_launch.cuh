@@ -2,10 +2,12 @@
 // closely (norm, product, cache), as programmatic dependents: a kernel's blocks
 // may start while the last blocks of the one before it in the stream finish, and
 // set up what touches no memory that those may still write or read; before_memory()
-// then waits until they are done and their writes are visible. Grids of more than 64
-// blocks an SM start in the ordinary way: under the last tiles of a product, a norm of
-// 65536 rows that started early made both take 550 us instead of 505, while the norm
-// and the reading back of 4099 rows gained 4.8 us of 28.6.
+// then waits until they are done and their writes are visible. What such a kernel reads
+// may thus be written while it already runs: its pointers must not promise otherwise
+// (__restrict__, ld.global.nc, __ldg), or the compiler could read ahead of the wait.
+// Grids of more than 64 blocks an SM start in the ordinary way: under the last tiles of a
+// product, a norm of 65536 rows that started early made both take 550 us instead of 505,
+// while the norm and the reading back of 4099 rows gained 4.8 us of 28.6.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -528,9 +528,8 @@ struct Bytes {
 
 template <class T, int V, int U>
 __global__ void __launch_bounds__(256, U == 1 ? 8 : V <= 4 ? 5 : 6)
-read_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t nslots,
-            const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr, int groups,
-            int gdim, int dim) {
+read_kernel(const int8_t* q, int64_t ldq, const float* scale, int64_t nslots, const int64_t* slots, T* out, int64_t ldo,
+            int64_t rows, int tpr, int groups, int gdim, int dim) {
     let_next_start();
     before_memory();
     const int per = 256 / tpr;
@@ -594,9 +593,8 @@ __device__ __noinline__ uint32_t word_edge(const int8_t* p, const int8_t* first,
 // bound by instructions.
 template <class T, bool WALK>
 __global__ void __launch_bounds__(256)
-read_odd_kernel(const int8_t* __restrict__ q, int64_t ldq, const int8_t* __restrict__ end, const float* __restrict__ scale,
-                int64_t nslots, const int64_t* __restrict__ slots, T* __restrict__ out, int64_t ldo, int64_t rows, int tpr,
-                int groups, int gdim, int dim) {
+read_odd_kernel(const int8_t* q, int64_t ldq, const int8_t* end, const float* scale, int64_t nslots,
+                const int64_t* slots, T* out, int64_t ldo, int64_t rows, int tpr, int groups, int gdim, int dim) {
     constexpr int V = 32 / (int)sizeof(T);
     let_next_start();
     before_memory();

@@ -1,0 +1,112 @@
+"""The 8-bit row operators on the paths that large or oddly placed rows take, and what their kernels and calls may assume."""
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "jhq_gpu_b200", "csrc")
+gpu = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def _randn(seed, *shape):
+    return torch.randn(*shape, generator=_gen(seed), device="cuda")
+
+
+def _rows(values, ld, dtype, offset=0):
+    """`values` as rows `ld` apart, the first `offset` elements behind a boundary."""
+    n, d = values.shape
+    buf = torch.zeros(n * ld + offset + d, dtype=dtype, device="cuda")
+    out = buf.as_strided((n, d), (ld, 1), offset)
+    out.copy_(values)
+    return out
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+# ---- kernels that start while the one before them ends ------------------------------------------------------------
+
+@pytest.mark.parametrize("name", ["q8_rows.cu", "q8_matmul.cu"])
+def test_kernels_promise_nothing_about_what_they_read(name):
+    """A kernel that starts before its predecessor's writes are done must not tell the compiler that what it reads is never
+    written: loads of such memory may be moved above the wait, or go past the coherent caches."""
+    with open(os.path.join(CSRC, name)) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert "before_memory();" in code
+    for promise in ("__restrict__", "__restrict", ".nc.", "__ldg", "ld.const"):
+        assert promise not in code, promise
+
+
+def _slots_as_rows(slots):
+    """An 8-bit row that reads back, in float32, as the bits of the int64s `slots` (0 .. 127): scale 2^-149, a low and a
+    high word each."""
+    q = torch.zeros(1, 2 * len(slots), dtype=torch.int8, device="cuda")
+    q[0, ::2] = slots.to(torch.int8)
+    return q, torch.tensor([2.0 ** -149], device="cuda")
+
+
+@gpu
+@pytest.mark.parametrize("n,groups,gdim,odd", [(3, 2, 64, 0), (300, 16, 128, 0), (20000, 2, 512, 0), (20000, 1, 1000, 0), (20001, 1, 1004, 0),
+                                               (5000, 3, 333, 0), (20000, 7, 9, 0), (300, 1, 256, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_reads_wait_for_values_scales_and_slots(jhq, n, groups, gdim, odd, dtype):
+    """The cache is written, the slots are written, and both are read, each by the kernel right before: several rows a
+    thread and one, whole and odd rows. Call by call with waits, and without."""
+    d, room = groups * gdim, 120
+    q = torch.zeros(room, d + odd, dtype=torch.int8, device="cuda")[:, odd:]
+    scale = torch.zeros(room, groups, device="cuda")
+    slots = torch.zeros(n, dtype=torch.int64, device="cuda")
+    out = torch.empty(n, d, dtype=dtype, device="cuda")
+    cache = jhq.Q8Rows.of(q, scale, groups=groups)
+    data = [(_randn(i, room, d).to(dtype), _slots_as_rows(torch.randint(0, room, (n,), generator=_gen(50 + i), device="cuda"))) for i in range(8)]
+
+    def chain(x, rows, wait):
+        for call in (lambda: jhq.q8_write(jhq.View.of(x), cache, stream=_stream()),
+                     lambda: jhq.q8_read(jhq.Q8Rows.of(*rows), jhq.View.of(slots.view(torch.float32).view(1, -1)), stream=_stream()),
+                     lambda: jhq.q8_read(cache, jhq.View.of(out), slots=slots.data_ptr(), stream=_stream())):
+            call()
+            if wait:
+                torch.cuda.synchronize()
+        return out.clone()
+
+    want = []
+    for x, rows in data:
+        want.append(chain(x, rows, True))
+        at = rows[0][0, ::2].long()
+        assert torch.equal(slots, at)
+        back = (q.float().view(room, groups, gdim) * scale[:, :, None]).view(room, d).to(dtype)
+        assert torch.equal(want[-1], back[at])
+    for _ in range(4):
+        got = [chain(x, rows, False) for x, rows in data]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("t,d,n", [(1, 999, 512), (33, 999, 130), (700, 1001, 300)])
+def test_products_of_packed_rows_wait_for_them(jhq, t, d, n):
+    """Rows that follow one another at odd addresses, read by the product right behind the norm that writes them, and
+    behind the call that writes the weights."""
+    q, scale = torch.empty(t, d, dtype=torch.int8, device="cuda"), torch.empty(t, device="cuda")
+    w, ws = torch.empty(n, d, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+    out = torch.empty(t, n, device="cuda")
+    data = [(_randn(i, t, d) * (i + 1), _randn(90 + i, n, d)) for i in range(10)]
+
+    def chain(x, y, wait):
+        for call in (lambda: jhq.q8_rms_norm(jhq.View.of(x), jhq.Q8Rows.of(q, scale), stream=_stream()),
+                     lambda: jhq.q8_write(jhq.View.of(y), jhq.Q8Rows.of(w, ws), stream=_stream()),
+                     lambda: jhq.q8_matmul(jhq.Q8Rows.of(q, scale), jhq.Q8Rows.of(w, ws), jhq.View.of(out), stream=_stream())):
+            call()
+            if wait:
+                torch.cuda.synchronize()
+        return out.clone()
+
+    want = [chain(x, y, True) for x, y in data]
+    for _ in range(4):
+        assert all(torch.equal(chain(x, y, False), a) for (x, y), a in zip(data, want))
