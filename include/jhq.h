@@ -315,6 +315,9 @@ int jhq_q8_write(const jhq_view* x, const int64_t* slots, const jhq_q8_rows* cac
  * [0, cache->rows) reads as zeros. */
 int jhq_q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out, void* stream);
 
+/* The ordinal of the calling thread's current device, -2 if there is none. */
+int jhq_current_device(void);
+
 /* After the streams of the calls above have drained: JHQ_ETIMEDOUT (once) if a
  * bounded device wait of one of them on the current device gave up, so that its
  * output is not valid, else JHQ_OK. */

@@ -42,7 +42,7 @@ EXPORTED = [
     "jhq_search_device_probes", "jhq_sharded_create", "jhq_sharded_destroy",
     "jhq_sharded_train", "jhq_sharded_add", "jhq_sharded_search", "jhq_sharded_set_nprobe",
     "jhq_sharded_ntotal", "jhq_q8_rms_norm", "jhq_q8_matmul", "jhq_q8_write", "jhq_q8_read",
-    "jhq_q8_status",
+    "jhq_q8_status", "jhq_current_device",
 ]
 STAGES = ["rotate", "coarse+probes", "plan", "scan", "refine"]
 

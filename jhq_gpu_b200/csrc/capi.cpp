@@ -306,6 +306,13 @@ int jhq_q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* 
     return guarded([&] { jhq::q8_read(cache, slots, out, static_cast<cudaStream_t>(stream)); });
 }
 
+int jhq_current_device(void) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) return dev;
+    cudaGetLastError();                                  // the answer is the return value
+    return -2;
+}
+
 int jhq_q8_status(void) {
     return guarded([&] {
         if (jhq::q8_take_error()) jhq::fail(JHQ_ETIMEDOUT, "a bounded device wait of an 8-bit product gave up");

@@ -7,7 +7,8 @@ product with an 8-bit projection, and a cache that rows are written to in 8 bits
 
 A View or Q8Rows describes device memory and does not keep it alive; `of` takes any 2-D tensor with data_ptr(),
 shape, stride() and dtype, such as torch's. Calls are asynchronous on `stream` (a raw CUDA stream, as
-torch.cuda.current_stream().cuda_stream) on the current device; errors are those of the package.
+torch.cuda.current_stream().cuda_stream) on the current device; errors are those of the package. Memory that `of` found
+elsewhere (on the host, on another GPU) is refused by the call that is given it.
 """
 from __future__ import annotations
 
@@ -30,9 +31,8 @@ def _kind(dtype) -> int:
     return kind
 
 
-def _shape(t, what: str):
+def _shape(shape, stride, what: str):
     """rows, columns and row stride of a 2-D (or, as one row, 1-D) tensor."""
-    shape, stride = t.shape, t.stride()
     if len(shape) == 2:
         rows, cols = shape
         ld, step = stride
@@ -45,21 +45,50 @@ def _shape(t, what: str):
     return rows, cols, ld if rows > 1 else cols
 
 
+# A description's `place` says where `of` found its memory: the GPU's ordinal + 2, 1 for host memory, 0 if the tensor doesn't
+# say. It lies in the C structure's padding, which C does not look at.
+def _check_places(L, fn, *operands) -> None:
+    """Refuses operands, in fn's order, whose memory is known not to be the current device's."""
+    here = L.jhq_current_device() + 2
+    try:
+        for o in operands:
+            if o is not None and o.place != here and o.place:
+                break
+        else:
+            return
+    except AttributeError:                                # not a description: refused by ctypes as such
+        return
+    kinds = [k._type_ for k in fn.argtypes if k._type_ in (View, Q8Rows)]
+    if all(b is None or isinstance(b, k) for b, k in zip(operands, kinds)):   # else the same
+        raise ValueError(f"{fn.__name__[4:]}: an operand lies in " + ("host memory" if o.place == 1 else f"the memory of GPU {o.place - 2}")
+                         + (f"; the current device is GPU {here - 2}" if here >= 2 else "; there is no current device"))
+
+
 class View(C.Structure):
     """jhq_view: a matrix of floating-point rows in device memory."""
     _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64),
-                ("type", C.c_int)]
+                ("type", C.c_int), ("place", C.c_int)]
 
     @classmethod
     def of(cls, t) -> "View":
         kind = _TYPES.get(t.dtype)
-        return cls(t.data_ptr(), *_shape(t, "View"), _kind(t.dtype) if kind is None else kind)
+        shape, stride = t.shape, t.stride()
+        if len(shape) == 2 and stride[1] == 1:            # the common matrix
+            rows, cols = shape
+            ld = stride[0] if rows > 1 else cols
+        else:
+            rows, cols, ld = _shape(shape, stride, "View")
+        try:
+            place = t.get_device() + 2
+        except AttributeError:
+            place = 0
+        return cls(t.data_ptr(), rows, cols, ld, _kind(t.dtype) if kind is None else kind, place)
 
 
 class Q8Rows(C.Structure):
     """jhq_q8_rows: a matrix of 8-bit rows in device memory, one float32 scale for each group of a row."""
     _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("rows", C.c_int64), ("dim", C.c_int64),
-                ("ld", C.c_int64), ("groups", C.c_int)]
+                ("ld", C.c_int64), ("groups", C.c_int), ("place", C.c_int)]
 
     @classmethod
     def of(cls, q, scale, groups: int = 1) -> "Q8Rows":
@@ -68,10 +97,21 @@ class Q8Rows(C.Structure):
             if str(q.dtype) not in ("torch.int8", "int8") or str(scale.dtype) not in ("torch.float32", "float32"):
                 raise ValueError(f"Q8Rows: int8 values and float32 scales are needed, got {q.dtype} and {scale.dtype}")
             _PAIRS.add((q.dtype, scale.dtype))
-        rows, dim, ld = _shape(q, "Q8Rows")
+        shape, stride = q.shape, q.stride()
+        if len(shape) == 2 and stride[1] == 1:            # the common matrix
+            rows, dim = shape
+            ld = stride[0] if rows > 1 else dim
+        else:
+            rows, dim, ld = _shape(shape, stride, "Q8Rows")
         if scale.numel() != rows * groups or not scale.is_contiguous():
             raise ValueError(f"Q8Rows: {rows} x {groups} packed scales are needed")
-        return cls(q.data_ptr(), scale.data_ptr(), rows, dim, ld, groups)
+        try:
+            place = q.get_device() + 2
+            if scale.get_device() + 2 != place:
+                raise ValueError("Q8Rows: values and scales must be on one device")
+        except AttributeError:
+            place = 0
+        return cls(q.data_ptr(), scale.data_ptr(), rows, dim, ld, groups, place)
 
 
 def _declare(L: C.CDLL) -> None:
@@ -81,28 +121,45 @@ def _declare(L: C.CDLL) -> None:
     L.jhq_q8_write.argtypes = [v, p, r, p]
     L.jhq_q8_read.argtypes = [r, p, v, p]
     L.jhq_q8_status.argtypes = []
+    L.jhq_current_device.argtypes = []
 
 
 def q8_rms_norm(x: View, out: Q8Rows, weight: Optional[View] = None, residual: Optional[View] = None,
                 residual_out: Optional[View] = None, eps: float = 1e-6, stream: int = 0) -> None:
     """out = 8-bit rows of h * weight / sqrt(mean(h^2) + eps), h = x + residual; residual_out = h."""
-    _J._check(_J.load_library().jhq_q8_rms_norm(x, residual, weight, eps, residual_out, out, stream))
+    L = _J._lib or _J.load_library()
+    _check_places(L, L.jhq_q8_rms_norm, x, residual, weight, residual_out, out)
+    rc = L.jhq_q8_rms_norm(x, residual, weight, eps, residual_out, out, stream)
+    if rc:
+        _J._check(rc)
 
 
 def q8_matmul(x: Q8Rows, w: Q8Rows, out: View, bias: Optional[View] = None, stream: int = 0) -> None:
     """out[t][n] = (sum_k x.q[t][k] w.q[n][k]) * x.scale[t] * w.scale[n] + bias[n], the sum exact."""
-    _J._check(_J.load_library().jhq_q8_matmul(x, w, bias, out, stream))
+    L = _J._lib or _J.load_library()
+    _check_places(L, L.jhq_q8_matmul, x, w, bias, out)
+    rc = L.jhq_q8_matmul(x, w, bias, out, stream)
+    if rc:
+        _J._check(rc)
 
 
 def q8_write(x: View, cache: Q8Rows, slots: Optional[int] = None, stream: int = 0) -> None:
     """Row i of x, quantised, to row slots[i] of the cache (slots: a device pointer to int64s; None: row i).
     Slots outside the cache (-1) are skipped."""
-    _J._check(_J.load_library().jhq_q8_write(x, slots, cache, stream))
+    L = _J._lib or _J.load_library()
+    _check_places(L, L.jhq_q8_write, x, cache)
+    rc = L.jhq_q8_write(x, slots, cache, stream)
+    if rc:
+        _J._check(rc)
 
 
 def q8_read(cache: Q8Rows, out: View, slots: Optional[int] = None, stream: int = 0) -> None:
     """Row slots[i] of the cache into row i of out, as scale * q; slots outside the cache read as zeros."""
-    _J._check(_J.load_library().jhq_q8_read(cache, slots, out, stream))
+    L = _J._lib or _J.load_library()
+    _check_places(L, L.jhq_q8_read, cache, out)
+    rc = L.jhq_q8_read(cache, slots, out, stream)
+    if rc:
+        _J._check(rc)
 
 
 def q8_check_status() -> None:

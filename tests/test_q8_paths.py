@@ -110,3 +110,61 @@ def test_products_of_packed_rows_wait_for_them(jhq, t, d, n):
     want = [chain(x, y, True) for x, y in data]
     for _ in range(4):
         assert all(torch.equal(chain(x, y, False), a) for (x, y), a in zip(data, want))
+
+
+# ---- operands that are not the current device's (no GPU is touched) ---------------------------------------------------
+
+class _Elsewhere:
+    """As much of a tensor as a description takes, on GPU 7; nothing is behind its address."""
+
+    def __init__(self, rows, cols, dtype):
+        self.shape, self.dtype = (rows, cols), dtype
+
+    def stride(self):
+        return self.shape[1], 1
+
+    def data_ptr(self):
+        return 4096
+
+    def get_device(self):
+        return 7
+
+    def numel(self):
+        return self.shape[0] * self.shape[1]
+
+    def is_contiguous(self):
+        return True
+
+
+def _operands(jhq, view, q8):
+    """Each call with every operand made by view(rows, cols) or q8(rows, dim)."""
+    return [(jhq.q8_rms_norm, (view(4, 64), q8(4, 64)), {}),
+            (jhq.q8_matmul, (q8(4, 64), q8(8, 64), view(4, 8)), {}),
+            (jhq.q8_write, (view(4, 64), q8(9, 64)), {}),
+            (jhq.q8_read, (q8(9, 64), view(4, 64)), {})]
+
+
+@pytest.mark.parametrize("call", range(4))
+def test_memory_elsewhere_is_refused(jhq, call):
+    raw_view, raw_q8 = (lambda n, d: jhq.View(4096, n, d, d, 0)), (lambda n, d: jhq.Q8Rows(4096, 8192, n, d, d, 1))
+    host_view = lambda n, d: jhq.View.of(torch.zeros(n, d))  # noqa: E731
+    host_q8 = lambda n, d: jhq.Q8Rows.of(torch.zeros(n, d, dtype=torch.int8), torch.zeros(n))  # noqa: E731
+    far_view = lambda n, d: jhq.View.of(_Elsewhere(n, d, torch.float32))  # noqa: E731
+    far_q8 = lambda n, d: jhq.Q8Rows.of(_Elsewhere(n, d, torch.int8), _Elsewhere(n, 1, torch.float32))  # noqa: E731
+    for where, v, r in (("host memory", host_view, host_q8), ("GPU 7", far_view, far_q8)):
+        for view, q8 in ((v, r), (v, raw_q8), (raw_view, r)):
+            f, args, kw = _operands(jhq, view, q8)[call]
+            with pytest.raises(ValueError, match=where):
+                f(*args, **kw)
+    with pytest.raises(ValueError, match="one device"):
+        jhq.Q8Rows.of(_Elsewhere(4, 64, torch.int8), torch.zeros(4))
+
+
+@pytest.mark.parametrize("operand", ["weight", "residual", "residual_out", "bias"])
+def test_optional_operands_elsewhere_are_refused(jhq, operand):
+    x, out = jhq.View(4096, 1, 64, 64, 0), jhq.Q8Rows(4096, 8192, 1, 64, 64, 1)
+    with pytest.raises(ValueError, match="host memory"):
+        if operand == "bias":
+            jhq.q8_matmul(out, out, jhq.View(4096, 1, 1, 1, 0), bias=jhq.View.of(torch.zeros(1, 1)))
+        else:
+            jhq.q8_rms_norm(x, out, **{operand: jhq.View.of(torch.zeros(1, 64))})
