@@ -67,7 +67,7 @@ def main(n=20000, nq=256, hidden=512, dim=128, k=10, seed=0):
     index.search_device(query.data_ptr(), nq, k, dists.data_ptr(), ids.data_ptr(), stream())
     found = torch.empty(nq * k, dim, device="cuda")           # a missing result's id is -1 and reads as zeros
     slots = ids.long().view(-1)                               # lives until the read has run
-    J.q8_read(J.Q8Rows.of(kept, kept_scale), J.View.of(found), slots=slots.data_ptr(), stream=stream())
+    J.q8_read(J.Q8Rows.of(kept, kept_scale), J.View.of(found), slots=slots, stream=stream())
     score = (found.view(nq, k, dim) * query[:, None]).sum(2)
     first = ids.long().gather(1, score.argmax(1, keepdim=True))[:, 0]
     torch.cuda.current_stream().synchronize()

@@ -64,6 +64,22 @@ def _check_places(L, fn, *operands) -> None:
                          + (f"; the current device is GPU {here - 2}" if here >= 2 else "; there is no current device"))
 
 
+def _slots(L, slots, v):
+    """The address that C takes: of a tensor, once it is known to be an int64 of the current device for each row of v; else as given."""
+    if slots is None or not hasattr(slots, "data_ptr"):
+        return slots
+    rows = v.rows
+    if str(slots.dtype) not in ("torch.int64", "int64"):
+        raise ValueError(f"slots: int64s are needed, got {slots.dtype}")
+    if tuple(slots.shape) != (rows,) or (rows > 1 and slots.stride()[0] != 1):
+        raise ValueError(f"slots: {rows} values that follow one another are needed, got a shape of {tuple(slots.shape)}"
+                         f" with strides {tuple(slots.stride())}")
+    here = L.jhq_current_device()
+    if hasattr(slots, "get_device") and slots.get_device() != here:
+        raise ValueError("slots: not in the memory of " + (f"the current device, GPU {here}" if here >= 0 else "a current device"))
+    return slots.data_ptr()
+
+
 class View(C.Structure):
     """jhq_view: a matrix of floating-point rows in device memory."""
     _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64),
@@ -143,21 +159,22 @@ def q8_matmul(x: Q8Rows, w: Q8Rows, out: View, bias: Optional[View] = None, stre
         _J._check(rc)
 
 
-def q8_write(x: View, cache: Q8Rows, slots: Optional[int] = None, stream: int = 0) -> None:
-    """Row i of x, quantised, to row slots[i] of the cache (slots: a device pointer to int64s; None: row i).
-    Slots outside the cache (-1) are skipped."""
+def q8_write(x: View, cache: Q8Rows, slots=None, stream: int = 0) -> None:
+    """Row i of x, quantised, to row slots[i] of the cache (None: row i). slots is a tensor of as many int64s as x has
+    rows, or their device address, which is taken unseen; slots outside the cache (-1) are skipped."""
     L = _J._lib or _J.load_library()
     _check_places(L, L.jhq_q8_write, x, cache)
-    rc = L.jhq_q8_write(x, slots, cache, stream)
+    rc = L.jhq_q8_write(x, _slots(L, slots, x), cache, stream)
     if rc:
         _J._check(rc)
 
 
-def q8_read(cache: Q8Rows, out: View, slots: Optional[int] = None, stream: int = 0) -> None:
-    """Row slots[i] of the cache into row i of out, as scale * q; slots outside the cache read as zeros."""
+def q8_read(cache: Q8Rows, out: View, slots=None, stream: int = 0) -> None:
+    """Row slots[i] of the cache into row i of out, as scale * q (slots as q8_write takes them, one for each row of out);
+    slots outside the cache read as zeros."""
     L = _J._lib or _J.load_library()
     _check_places(L, L.jhq_q8_read, cache, out)
-    rc = L.jhq_q8_read(cache, slots, out, stream)
+    rc = L.jhq_q8_read(cache, _slots(L, slots, out), out, stream)
     if rc:
         _J._check(rc)
 

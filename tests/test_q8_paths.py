@@ -168,3 +168,47 @@ def test_optional_operands_elsewhere_are_refused(jhq, operand):
             jhq.q8_matmul(out, out, jhq.View(4096, 1, 1, 1, 0), bias=jhq.View.of(torch.zeros(1, 1)))
         else:
             jhq.q8_rms_norm(x, out, **{operand: jhq.View.of(torch.zeros(1, 64))})
+
+
+class _Slots(_Elsewhere):
+    def __init__(self, n, dtype=torch.int64, step=1, shape=None, place=7):
+        super().__init__(n, 1, dtype)
+        self.shape, self._step, self._place = (n,) if shape is None else shape, step, place
+
+    def stride(self):
+        return (self._step,) * len(self.shape)
+
+    def get_device(self):
+        return self._place
+
+
+@pytest.mark.parametrize("slots,msg", [
+    (_Slots(4, torch.int32), "int64s are needed"), (_Slots(4, torch.float32), "int64s are needed"), (_Slots(3), "4 values"),
+    (_Slots(5), "4 values"), (_Slots(4, step=2), "4 values"), (_Slots(4, shape=(2, 2)), "4 values"), (_Slots(4), "not in the memory"),
+    (torch.zeros(4, dtype=torch.int64), "not in the memory")])
+def test_slots_that_do_not_fit_are_refused(jhq, slots, msg):
+    view, cache = jhq.View(4096, 4, 64, 64, 0), jhq.Q8Rows(4096, 8192, 9, 64, 64, 1)
+    with pytest.raises(ValueError, match=msg):
+        jhq.q8_write(view, cache, slots=slots)
+    with pytest.raises(ValueError, match=msg):
+        jhq.q8_read(cache, view, slots=slots)
+
+
+@gpu
+def test_slots_as_a_tensor_and_as_an_address(jhq):
+    q, scale = torch.zeros(9, 64, dtype=torch.int8, device="cuda"), torch.zeros(9, device="cuda")
+    cache, x = jhq.Q8Rows.of(q, scale), _randn(1, 4, 64)
+    slots = torch.tensor([8, -1, 0, 3], device="cuda")
+    outs = []
+    for given in (slots, slots.data_ptr()):
+        q.zero_()
+        scale.zero_()
+        jhq.q8_write(jhq.View.of(x), cache, slots=given, stream=_stream())
+        out = torch.empty(4, 64, device="cuda")
+        jhq.q8_read(cache, jhq.View.of(out), slots=given, stream=_stream())
+        outs.append(out)
+    assert torch.equal(*outs) and not outs[0][1].any() and outs[0][0].any()
+    with pytest.raises(ValueError, match="4 values"):
+        jhq.q8_read(cache, jhq.View.of(out), slots=slots[:3], stream=_stream())
+    with pytest.raises(ValueError, match="int64s"):
+        jhq.q8_write(jhq.View.of(x), cache, slots=slots.int(), stream=_stream())
