@@ -232,6 +232,9 @@ __device__ __forceinline__ float2 team_sum_max(float sum, float top, float2* red
     }
     return make_float2(sum, top);
 }
+// The power of two (2^-128 .. 2^126) that brings a positive h into 1/2 .. 1 (a subnormal one as near as it goes): no
+// product of it with a finite weight overflows then.
+__device__ __forceinline__ float to_unit(float h) { return ldexpf(1.0f, -max(ilogbf(h) + 1, -126)); }
 __device__ __forceinline__ bool is_finite(float a) { return (__float_as_uint(a) & 0x7fffffffu) < INF_BITS; }
 
 struct Args {
@@ -342,7 +345,7 @@ __global__ void __maxnreg__(EPT == 32 && (sizeof(T) == 4 || sizeof(R) == 4) ? 80
 #pragma unroll
         for (int i = 0; i < EPT; ++i) hm = max_nan(hm, h[i]);
         const float htop = team_sum_max<TEAM>(0.0f, hm, red[1]).y;
-        if (odd && htop > 0.0f && is_finite(htop)) by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
+        if (odd && htop > 0.0f && is_finite(htop)) by = to_unit(htop);
         gather(by);
         const float2 s2 = team_sum_max<TEAM>(sum, top, red[2]);
         top_g = s2.y;
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_co
             for (int j = threadIdx.x; j < a.d; j += LONG_THREADS) hm = max_nan(hm, h_of(j));
             const float htop = team_sum_max<0>(0.0f, hm, red[1]).y;
             if (htop > 0.0f && is_finite(htop)) {
-                by = ldexpf(1.0f, -min(max(ilogbf(htop), -126), 126));
+                by = to_unit(htop);
                 const float2 s2 = gather(by, red[2]);
                 top_g = s2.y;
                 step = (float)((double)top_g / (127.0 * sqrt((double)s2.x / a.d + (double)a.eps * by * by)));

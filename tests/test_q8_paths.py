@@ -8,6 +8,14 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "jhq_gpu_b200", "csrc")
 gpu = pytest.mark.gpu
+U = 2.0 ** -24                          # half a unit in the last place of float32, relative
+
+
+def _norm_tol(d):
+    """Of a normed row's step. A thread adds at most 32 squares in sequence, or a 1024th of a long row, and the team's
+    reductions at most 10 sums more; a square's h is rounded once: the sum of squares is within (max(32, d / 1024) + 13) U,
+    halved by the root. The root, the mean, eps, the two products and the largest |h w| add less than 8 U."""
+    return ((max(32, -(-d // 1024)) + 13) / 2 + 8) * U
 
 
 def _gen(seed):
@@ -212,3 +220,25 @@ def test_slots_as_a_tensor_and_as_an_address(jhq):
         jhq.q8_read(cache, jhq.View.of(out), slots=slots[:3], stream=_stream())
     with pytest.raises(ValueError, match="int64s"):
         jhq.q8_write(jhq.View.of(x), cache, slots=slots.int(), stream=_stream())
+
+
+# ---- a weight next to the largest float32 ------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("d", [64, 1024, 5003, 70000])
+@pytest.mark.parametrize("size", [1.5, 1.9, 3e30, 1.9e-30])
+def test_norm_whose_product_with_the_weight_leaves_the_range(jhq, d, size):
+    """h * w is beyond float32 where h is not yet divided by its norm; the normed row is not. What is rounded to 8 bits has
+    seen 6 roundings, and 1 / a, which is subnormal here, one to 2^-149: within 127 (6u + 2^-22) < 8e-5 of a step."""
+    x = torch.full((3, d), size, device="cuda")
+    x[:, ::3] *= -0.5
+    w = torch.full((d,), 1.5e38, device="cuda")
+    w[1::4] = 2.5e38
+    q, scale = torch.empty(3, d, dtype=torch.int8, device="cuda"), torch.empty(3, device="cuda")
+    jhq.q8_rms_norm(jhq.View.of(x), jhq.Q8Rows.of(q, scale), weight=jhq.View.of(w), eps=0.0, stream=_stream())
+    h = x.double()
+    y = h / h.square().mean(1, keepdim=True).sqrt() * w.double()
+    step = y.abs().amax(1, keepdim=True) / 127
+    assert float(y.abs().max()) < 3.4e38                       # else the row itself is not finite
+    assert torch.all((scale.double()[:, None] - step).abs() <= _norm_tol(d) * step)
+    assert torch.all((q.double() * step - y).abs() <= (0.5 + 8e-5) * step)
