@@ -242,3 +242,133 @@ def test_norm_whose_product_with_the_weight_leaves_the_range(jhq, d, size):
     assert float(y.abs().max()) < 3.4e38                       # else the row itself is not finite
     assert torch.all((scale.double()[:, None] - step).abs() <= _norm_tol(d) * step)
     assert torch.all((q.double() * step - y).abs() <= (0.5 + 8e-5) * step)
+
+
+# ---- the paths of many rows, ragged rows and rows off their boundaries -------------------------------------------------
+#
+# Tolerances: _norm_tol() for a step; what is rounded to 8 bits has seen at most 7 roundings, 127 * 7 U < 6e-5 of a step.
+
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
+
+
+def _check_q8(q, scale, y, step_tol):
+    step = y.abs().amax(-1, keepdim=True) / 127
+    assert torch.all((scale.double().view(step.shape) - step).abs() <= step_tol * step + 2.0 ** -149)
+    assert torch.all((q.double() * step - y).abs() <= (0.5 + 6e-5) * step + 2.0 ** -149)
+    assert int(q.min()) >= -127
+
+
+def _blank(rows, d, at, dtype, fill):
+    """`rows` rows of d at distance at[0], at[1] elements behind a boundary, and a check that nothing beside them changed."""
+    buf = torch.full((rows * at[0] + at[1],), fill, dtype=dtype, device="cuda")
+    view = buf.as_strided((rows, d), (at[0], 1), at[1])
+
+    def beside():
+        gap = buf[at[1]:].view(rows, at[0])[:, d:]
+        return bool((gap == fill).all()) and bool((buf[:at[1]] == fill).all())
+    return view, beside
+
+
+def _norm_and_check(jhq, rows, d, dtype, rtype, x_at, r_at, o_at, q_at):
+    """Each *_at: (distance of rows, elements behind a boundary) of x, residual, residual_out and q."""
+    x, w = _rows(_randn(1, rows, d) * 3, x_at[0], dtype, x_at[1]), (1 + 0.3 * _randn(2, d)).to(dtype)
+    (q, q_beside), scale = _blank(rows, d, q_at, torch.int8, 99), torch.full((rows,), -1.0, device="cuda")
+    h, kw = x.double(), {}
+    if rtype:
+        res = _rows(_randn(3, rows, d), r_at[0], rtype, r_at[1])
+        res_out, o_beside = _blank(rows, d, o_at, rtype, 7.0)
+        h = h + res.double()
+        kw = dict(residual=jhq.View.of(res), residual_out=jhq.View.of(res_out))
+    jhq.q8_rms_norm(jhq.View.of(x), jhq.Q8Rows.of(q, scale), weight=jhq.View.of(w), stream=_stream(), **kw)
+    y = h / (h.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+    _check_q8(q, scale, y, _norm_tol(d))
+    assert q_beside()
+    if rtype:
+        assert torch.equal(res_out, (x.float() + res.float()).to(rtype)) and o_beside()
+
+
+def _up(n, to):
+    return -(-n // to) * to
+
+
+TYPES = [(BF, BF), (BF, FL), (FL, FL), (HF, None), (FL, None), (HF, HF)]
+MANY = [(20001, 64), (20001, 100), (20001, 128), (20001, 130), (20001, 250), (20001, 256), (20001, 300), (20001, 500), (20001, 512), (20001, 600),
+        (20001, 1003), (20001, 1024), (9001, 2003), (9001, 2048), (4001, 5001), (2001, 9001), (701, 16001), (20, 20001)]
+
+
+@gpu
+@pytest.mark.parametrize("rows,d", MANY)
+@pytest.mark.parametrize("dtype,rtype", TYPES)
+def test_norm_of_many_rows_on_boundaries(jhq, rows, d, dtype, rtype):
+    ld = _up(d, 16)
+    _norm_and_check(jhq, rows, d, dtype, rtype, (ld, 0), (ld, 0), (ld, 0), (ld, 0))
+
+
+@gpu
+@pytest.mark.parametrize("rows,d", [(20001, 100), (20001, 1003), (9001, 2003), (20001, 512), (3, 1000), (5, 4001), (300, 777), (2001, 9001)])
+@pytest.mark.parametrize("dtype,rtype", TYPES)
+@pytest.mark.parametrize("odd", ["out", "q", "both", "out_shifted", "q_shifted"])
+def test_norm_with_outputs_off_their_boundaries(jhq, rows, d, dtype, rtype, odd):
+    ld, off = _up(d, 16), (d + 1 - d % 2, 0)
+    if "shifted" in odd:
+        off = (ld + 16, 5)
+    _norm_and_check(jhq, rows, d, dtype, rtype, (ld, 0), (ld, 0), off if odd[:3] == "out" or odd == "both" else (ld, 0),
+                    off if odd[0] == "q" or odd == "both" else (ld, 0))
+
+
+@gpu
+@pytest.mark.parametrize("rows,d", [(20001, 7), (20001, 100), (20001, 200), (9001, 300), (9001, 500), (4001, 700), (2001, 1500), (1001, 2900), (601, 6000),
+                                    (601, 9001)])
+@pytest.mark.parametrize("dtype,rtype,odd", [(t, r, odd) for t, r in TYPES for odd in ("x", "residual") if odd == "x" or r])
+def test_norm_of_many_rows_off_their_boundaries(jhq, rows, d, dtype, rtype, odd):
+    ld = _up(d, 16)
+    _norm_and_check(jhq, rows, d, dtype, rtype, (ld + 1, 1) if odd == "x" else (ld, 0), (ld, 0) if odd == "x" else (ld + 3, 1), (ld, 0), (ld, 0))
+
+
+@gpu
+@pytest.mark.parametrize("n,groups,gdim", [(20001, 1, 11), (20001, 1, 27), (20001, 1, 60), (20001, 1, 100), (20001, 1, 333), (20001, 1, 1003), (9001, 1, 2003),
+                                           (601, 1, 9001), (9001, 16, 128), (9001, 4, 16), (9001, 4, 32), (9001, 4, 64), (9001, 3, 40), (9001, 2, 520),
+                                           (9001, 5, 23), (2001, 2, 1501), (601, 2, 6001), (9001, 2, 1024)])
+@pytest.mark.parametrize("dtype", [FL, HF, BF])
+@pytest.mark.parametrize("odd", [False, True])
+def test_cache_of_many_rows(jhq, n, groups, gdim, dtype, odd):
+    d = groups * gdim
+    ld, off, room = _up(d, 16) + odd, int(odd), n + 37
+    x = _rows(_randn(4, n, d), ld, dtype, off)
+    q = _rows(torch.full((room, d), 99, device="cuda"), ld, torch.int8, off)
+    scale = torch.full((room, groups), -1.0, device="cuda")
+    slots = torch.randperm(room, generator=_gen(5), device="cuda")[:n]
+    slots[1], slots[n - 1] = -1, room
+    cache = jhq.Q8Rows.of(q, scale, groups=groups)
+    jhq.q8_write(jhq.View.of(x), cache, slots=slots, stream=_stream())
+    kept = (slots >= 0) & (slots < room)
+    at = slots[kept]
+    _check_q8(q[at].reshape(-1, gdim), scale[at].reshape(-1), x[kept].double().reshape(-1, gdim), 2 * U)
+    other = torch.ones(room, dtype=torch.bool, device="cuda")
+    other[at] = False
+    assert bool((q[other] == 99).all()) and bool((scale[other] == -1).all())
+    for many in (n, 3):
+        back = torch.randint(-1, room + 1, (many,), generator=_gen(6), device="cuda")
+        out = _rows(torch.full((many, d), 5.0, device="cuda"), ld, dtype, off)
+        jhq.q8_read(cache, jhq.View.of(out), slots=back, stream=_stream())
+        to = back.clamp(0, room - 1)
+        want = (q[to].float().view(-1, groups, gdim) * scale[to][:, :, None]).view(many, d).to(dtype)
+        want[(back < 0) | (back >= room)] = 0
+        assert torch.equal(out, want)
+
+
+@gpu
+@pytest.mark.parametrize("n,dim", [(80001, 128), (20001, 1000), (20001, 1004), (5001, 2048), (9501, 4000), (20003, 520)])
+@pytest.mark.parametrize("dtype", [FL, HF, BF])
+def test_reading_several_rows_a_thread(jhq, n, dim, dtype):
+    """Every load width of the aligned read, at row counts that end inside a thread's rows."""
+    room = 1000
+    q = _rows(torch.randint(-127, 128, (room, dim), generator=_gen(7), device="cuda"), _up(dim, 16), torch.int8)
+    scale = torch.rand(room, generator=_gen(8), device="cuda")
+    slots = torch.randint(-1, room + 1, (n,), generator=_gen(9), device="cuda")
+    out = torch.full((n, dim), 5.0, dtype=dtype, device="cuda")
+    jhq.q8_read(jhq.Q8Rows.of(q, scale), jhq.View.of(out), slots=slots, stream=_stream())
+    at = slots.clamp(0, room - 1)
+    want = (q.float() * scale[:, None]).to(dtype)[at]
+    want[(slots < 0) | (slots >= room)] = 0
+    assert torch.equal(out, want)
