@@ -109,19 +109,14 @@ __device__ __forceinline__ void load(const T* p, int left, float* out) {
     } else {
         left -= A == RAGGED ? V - 1 : 0;                   // whole pieces alone; mend() follows
         uint32_t v[B / 4];
-        if constexpr (B >= 16) {
+        static_assert(B % 16 == 0, "16-bit rows may have float32 weights and residuals, float32 rows only such");
 #pragma unroll
-            for (int i = 0; i < B / 16; ++i) {
-                const uint4* from = reinterpret_cast<const uint4*>(p) + i;
-                uint4 u;
-                if constexpr (A != FULL) load_if<STREAM>(left > 0, from, u);
-                else u = STREAM ? load16(from) : *from;
-                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
-            }
-        } else {
-            static_assert(B == 8, "four 16-bit weights or residuals of float32 rows");
-            const uint2 u = A == FULL || left > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
-            v[0] = u.x; v[1] = u.y;
+        for (int i = 0; i < B / 16; ++i) {
+            const uint4* from = reinterpret_cast<const uint4*>(p) + i;
+            uint4 u;
+            if constexpr (A != FULL) load_if<STREAM>(left > 0, from, u);
+            else u = STREAM ? load16(from) : *from;
+            v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
         }
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -162,8 +157,6 @@ __device__ __forceinline__ void put(T* p, int left, const float* in, bool odd) {
     if constexpr (B >= 16) {
 #pragma unroll
         for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
-    } else if constexpr (B == 8) {
-        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
     } else {
         p[0] = v[0];
     }
@@ -468,12 +461,14 @@ void launch_rows(const Args& a, cudaStream_t s) {
     const int d = a.d;
     // whether all rows, `each` values a thread, are on the SMs at once
     const auto fits = [&](int each) { return d > 256 && d <= each * MOST_THREADS && (int64_t)a.teams * ((d - 1) / each + 1) <= SMS * 1024; };
-    if (!NORM && d <= 16) return launch_team<T, R, 2, 8, A, NORM>(a, s);
-    if (!NORM && d <= 32) return launch_team<T, R, 4, 8, A, NORM>(a, s);
+    if constexpr (!NORM) {                                 // short groups, of which a cache has many
+        if (d <= 16) return launch_team<T, R, 2, 8, A, NORM>(a, s);
+        if (d <= 32) return launch_team<T, R, 4, 8, A, NORM>(a, s);
+        if (d <= 64) return launch_team<T, R, A == SINGLE ? 4 : 2, A == SINGLE ? 16 : 32, A, NORM>(a, s);
+    }
     if (fits(8)) return launch_block<T, R, 8, A, NORM>(a, s);
     if (fits(16)) return launch_block<T, R, 16, A, NORM>(a, s);
     if constexpr (A == SINGLE) {
-        if (!NORM && d <= 64) return launch_team<T, R, 4, 16, A, NORM>(a, s);
         if (d <= 128) return launch_team<T, R, 8, 16, A, NORM>(a, s);
         if (d <= 256) return launch_team<T, R, 16, 16, A, NORM>(a, s);
         if (d <= 512) return launch_team<T, R, 32, 16, A, NORM>(a, s);
@@ -482,7 +477,6 @@ void launch_rows(const Args& a, cudaStream_t s) {
         if (d <= 4096) return launch_team<T, R, 256, 16, A, NORM>(a, s);
         if (d <= 8192) return launch_team<T, R, 512, 16, A, NORM>(a, s);
     } else {
-        if (!NORM && d <= 64) return launch_team<T, R, 2, 32, A, NORM>(a, s);
         if (d <= 128) return launch_team<T, R, 4, 32, A, NORM>(a, s);
         if (d <= 256) return launch_team<T, R, 8, 32, A, NORM>(a, s);
         if (d <= 512) return launch_team<T, R, 16, 32, A, NORM>(a, s);
@@ -579,8 +573,7 @@ read_kernel(const int8_t* q, int64_t ldq, const float* scale, int64_t nslots, co
     }
 }
 
-// The four bytes at p (any address) of a buffer [first, end): from the two aligned words that hold them, where these lie
-// inside, else byte by byte, zeros outside.
+// The four bytes at p (any address) of a buffer [first, end), byte by byte, zeros outside.
 __device__ __noinline__ uint32_t word_edge(const int8_t* p, const int8_t* first, const int8_t* end) {
     uint32_t v = 0;
 #pragma unroll 1
@@ -733,11 +726,10 @@ void q8_rms_norm(const jhq_view* x, const jhq_view* residual, const jhq_view* we
         constexpr int V = 16 / (int)sizeof(T);
         auto go = [&](auto r) {
             using R = decltype(r);
-            const int rb = std::min(16, V * (int)sizeof(R));
-            const bool vec = on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) && on_bytes(a.res, a.ldr, sizeof(R), rb, x->rows) &&
+            const bool vec = on_bytes(a.x, a.ldx, sizeof(T), 16, x->rows) && on_bytes(a.res, a.ldr, sizeof(R), 16, x->rows) &&
                              (uintptr_t)a.weight % 16 == 0;
             a.odd_q = !on_bytes(a.q, a.ldq, 1, V, x->rows);
-            a.odd_out = !on_bytes(a.res_out, a.ldo, sizeof(R), rb, x->rows);
+            a.odd_out = !on_bytes(a.res_out, a.ldo, sizeof(R), 16, x->rows);
             if (!vec) launch_rows<T, R, SINGLE, true>(a, s);
             else if (a.d % V == 0) launch_rows<T, R, WHOLE, true>(a, s);
             else launch_rows<T, R, RAGGED, true>(a, s);
@@ -790,9 +782,9 @@ void q8_read(const jhq_q8_rows* cache, const int64_t* slots, const jhq_view* out
     if (out->rows == 0) return;
     by_type(out->type, [&](auto t) {
         using T = decltype(t);
-        if (!try_read<T, 32 / (int)sizeof(T)>(cache, slots, out, s) && !try_read<T, 8>(cache, slots, out, s) &&
-            !try_read<T, 4>(cache, slots, out, s))
-            read_odd<T>(cache, slots, out, s);
+        bool done = try_read<T, 32 / (int)sizeof(T)>(cache, slots, out, s);
+        if constexpr (sizeof(T) == 2) done = done || try_read<T, 8>(cache, slots, out, s);
+        if (!done && !try_read<T, 4>(cache, slots, out, s)) read_odd<T>(cache, slots, out, s);
     });
     JHQ_LAUNCH_CHECK();
     count_launch();
