@@ -66,7 +66,7 @@ def _check_places(L, fn, *operands) -> None:
 
 def _slots(L, slots, v):
     """The address that C takes: of a tensor, once it is known to be an int64 of the current device for each row of v; else as given."""
-    if slots is None or not hasattr(slots, "data_ptr"):
+    if not hasattr(slots, "data_ptr"):
         return slots
     rows = v.rows
     if str(slots.dtype) not in ("torch.int64", "int64"):
@@ -137,6 +137,7 @@ def _declare(L: C.CDLL) -> None:
     L.jhq_q8_write.argtypes = [v, p, r, p]
     L.jhq_q8_read.argtypes = [r, p, v, p]
     L.jhq_q8_status.argtypes = []
+    L.jhq_current_device = C.PyDLL(L._name).jhq_current_device   # too quick to hand the interpreter's lock back
     L.jhq_current_device.argtypes = []
 
 
@@ -164,7 +165,7 @@ def q8_write(x: View, cache: Q8Rows, slots=None, stream: int = 0) -> None:
     rows, or their device address, which is taken unseen; slots outside the cache (-1) are skipped."""
     L = _J._lib or _J.load_library()
     _check_places(L, L.jhq_q8_write, x, cache)
-    rc = L.jhq_q8_write(x, _slots(L, slots, x), cache, stream)
+    rc = L.jhq_q8_write(x, slots if slots is None or type(slots) is int else _slots(L, slots, x), cache, stream)
     if rc:
         _J._check(rc)
 
@@ -174,7 +175,7 @@ def q8_read(cache: Q8Rows, out: View, slots=None, stream: int = 0) -> None:
     slots outside the cache read as zeros."""
     L = _J._lib or _J.load_library()
     _check_places(L, L.jhq_q8_read, cache, out)
-    rc = L.jhq_q8_read(cache, _slots(L, slots, out), out, stream)
+    rc = L.jhq_q8_read(cache, slots if slots is None or type(slots) is int else _slots(L, slots, out), out, stream)
     if rc:
         _J._check(rc)
 
