@@ -5,9 +5,11 @@
 // then waits until they are done and their writes are visible. What such a kernel reads
 // may thus be written while it already runs: its pointers must not promise otherwise
 // (__restrict__, ld.global.nc, __ldg), or the compiler could read ahead of the wait.
-// Grids of more than 64 blocks an SM start in the ordinary way: under the last tiles of a
-// product, a norm of 65536 rows that started early made both take 550 us instead of 505,
-// while the norm and the reading back of 4099 rows gained 4.8 us of 28.6.
+// Grids of more than 64 blocks an SM start in the ordinary way. A norm (one block a row) and
+// the product that follows it, in turn, took with no early start / this limit / early starts
+// alone: 4096 rows of 4096 44.9 / 45.1 / 45.1 us, 8192 73.1 / 75.4 / 75.3, 12288 102.5 / 100.9 /
+// 105.2, 32768 239 / 238 / 259, 65536 rows of 2048 210 / 208 / 230. The norm and its reading
+// back: 2048 rows of 4096 17.6 / 17.2 / 17.2, 4096 34.0 / 33.0 / 33.0, 32768 215 / 215 / 213.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -242,9 +242,10 @@ __device__ __forceinline__ bool epilogue_wait(uint32_t bar, uint32_t parity, boo
 // a 128-row MMA empty and 128 channels fill it with bytes that are read once anyway.
 // Bound by the weights' bytes for long rows, by launch, ring and epilogue (3 to 5 us) for
 // short ones. Measured: 1 x 8192 x 8192 13.7 us (4.9 TB/s, 0.75 of a copy's rate), 64 x 8192
-// x 8192 16.2 us (4.2 TB/s), 1 x 1024 x 4096 3.8 us, 256 x 1024 x 4096 7.6 us; from rows at
-// odd addresses, bound by the loads' latency, 1000 x 999 x 1001 14.0 us, 4001 x 4001 x 4001
-// 408 us (314 TOP/s).
+// x 8192 16.3 us (4.2 TB/s), 16 x 16384 x 16384 43.5 us (6.2 TB/s), 1 x 1024 x 4096 3.9 us,
+// 256 x 1024 x 4096 7.7 us; from rows at odd addresses, bound by the loads' latency, 1000 x 999
+// x 1001 14.1 us, 4001 x 4001 x 4001 418 us (306 TOP/s, a tenth of the aligned rate; the kernel
+// of 128 tokens spills 40 bytes a thread).
 constexpr int BM = 128, BK = 128;
 constexpr int LOADERS = 256;                               // threads of the epilogue, which load where TMA cannot
 constexpr int LOAD_GROUPS = 2;                             // as many again, which load every other stage
@@ -536,10 +537,11 @@ panel_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 // and a tile's epilogue runs under the next tile's products. Tokens are the rows
 // here so that a thread has neighbouring outputs of one token (5 instructions an
 // output; 32 with channels as rows and 2-byte stores). Bound by the tensor cores, and
-// over seconds by the power limit. Measured: 32768 x 8192 x 8192 1270 us in a burst (3.46
-// POP/s; twice the bfloat16 rate of a library product is 3.32), 1556 us sustained (2.83;
-// twice its sustained rate is 2.77); 8192 x 4096 x 4096 87 us (3.14, tensor pipe 89%
-// active); 65536 x 1024 x 4096 184 us; 65536 x 512 x 512, bound by outputs, 30 us.
+// over seconds by the power limit. Measured: 32768 x 8192 x 8192 1270 to 1390 us in a burst,
+// by the GPU (3.46 to 3.16 POP/s; twice the bfloat16 rate of a library product is 3.32),
+// 1530 to 1650 us sustained (2.87 to 2.67; twice its sustained rate is 2.77); 8192 x 4096 x
+// 4096 88 us (3.14, tensor pipe 89% active); 65536 x 1024 x 4096 185 us; 65536 x 512 x 512,
+// bound by outputs, 30 us.
 constexpr int PAIR_EPI_WARPS = 8;
 constexpr int PAIR_THREADS = 96 + 32 * PAIR_EPI_WARPS;
 constexpr int RASTER = 8;                                  // tiles of tokens walked together
@@ -886,11 +888,14 @@ void pairs(const jhq_q8_rows* x, const jhq_q8_rows* w, const Epilogue& e, cudaSt
               (int)x->dim, (int)mt, (int)nt, e);
 }
 
-// Which kernel, tile and split: the least of the microseconds that these costs give, fitted to timings of launches in
-// a graph. A K block of 128 bytes takes 0.14 us in a panel (barriers and issue) and in a pair with 128 channels, 0.272 us
+// Which kernel, tile and split: the least of the costs below, fitted to microseconds of launches in a graph. They leave the
+// operands' bytes out, and where those bind only order the choices (64 x 8192 x 8192 costs 9.8 and takes 16.3 us, 16 x 16384 x
+// 16384 20.9 and 43.5). A K block of 128 bytes takes 0.14 us in a panel (barriers and issue) and in a pair with 128 channels, 0.272 us
 // in one with 256 (the MMAs), more as all pairs draw on L2; the rest is launch, filling the ring, joining slices and the
 // epilogue. Best panel / pair of 128 / pair of 256, in us: 256 x 1024 x 4096 7.5 / 8.9 / 14.3; 512 x 1024 x 1024
-// 5.2 / 5.5 / 7.8; 256 x 4096 x 4096 10.1 / 9.3 / 14.7; 8192 x 4096 x 4096 236 / 99 / 86.
+// 5.2 / 5.5 / 7.8; 256 x 4096 x 4096 10.1 / 9.3 / 14.7; 8192 x 4096 x 4096 236 / 99 / 86. Above 2048 tokens only pairs are
+// looked at: the panels' costs are too low there (4096 x 512 x 4096: panels cost 10.8 and take 13.6 us, pairs 10.8 and 10.7).
+// The limit loses where few channels meet long rows (4096 x 128 x 16384: panels would take 18.3 us, pairs take 26.6).
 struct Plan {
     int tile, split;                                       // split 0: pairs
     double us;
@@ -926,7 +931,7 @@ Plan plan(const jhq_q8_rows* x, const jhq_q8_rows* w) {
 }
 // Rows that TMA cannot fetch: panels, whose loader threads bind, who bring 128 + tile rows for 128 x tile products.
 // 1 x 4001 x 4001 in tiles of 16 took 32 / 18 / 11.5 us in 1 / 2 / 4 slices, 1000 x 999 x 1001 in tiles of 64 14.0 us, of
-// 128 in two slices 15.4 us, 4001 x 4001 x 4001 in tiles of 64 555 us, of 128 428 us.
+// 128 in two slices 15.4 us, 4001 x 4001 x 4001 in tiles of 64 555 us, of 128 418 us.
 Plan plan_unaligned(const jhq_q8_rows* x, const jhq_q8_rows* w) {
     Plan best{128, 1, 1e30};
     const double block[4] = {0.85, 0.85, 1.0, 1.5}, first[4] = {4.8, 5.0, 5.4, 6.5};

@@ -258,10 +258,12 @@ constexpr int SMS = 148;
 // threads as they need (TEAM = 0) or, for single values, of TEAM, so that their
 // addresses differ by constants (20000 x 1001 in bfloat16, packed: 84 us without, 60 us
 // with). Registers are held to 64, and to 80 where a thread holds 32 float32 values or
-// residuals.
+// residuals, for the whole pieces of most rows; the RAGGED norms of 32 values spill 130 to
+// 220 bytes a thread under it in 16-bit types (20000 x 1003 in padded rows: 69 us).
 // Measured: norm of 65536 x 4096 in bfloat16 with its residual 299 us (6.28 TB/s, 0.96 of
-// a copy's rate), with a float32 residual 476 us (6.20 TB/s); 1 x 4096 2.6 us; 65536 x 1024
-// 78 us (6.02 TB/s); cache write of 65536 x 16 x 128 in bfloat16 71 us (5.65 TB/s).
+// a copy's rate), with a float32 residual 476 us (6.20 TB/s); 1 x 4096 2.5 us; 65536 x 1024
+// 78 us (6.03 TB/s); cache write of 65536 x 16 x 128 in bfloat16 71 us (5.64 TB/s), of odd
+// groups, value by value, 30000 x 7 x 333 95 us (2.21 TB/s).
 constexpr int SHARED_BLOCK = 128, MOST_THREADS = 512;
 template <class T, class R, int TEAM, int EPT, Access A, bool NORM>
 __global__ void __maxnreg__(EPT == 32 && (sizeof(T) == 4 || sizeof(R) == 4) ? 80 : 64) rows_kernel(const __grid_constant__ Args a) {
@@ -379,7 +381,7 @@ __global__ void __maxnreg__(EPT == 32 && (sizeof(T) == 4 || sizeof(R) == 4) ? 80
 
 // Rows longer than a block's registers: the row is read twice (thrice near the
 // ends of float32's range), value by value: bound by instructions. Measured: norm of 4096 x
-// 32768 in bfloat16 335 us (2.8 TB/s).
+// 32768 in bfloat16 336 us (2.8 TB/s).
 constexpr int LONG_THREADS = 1024;
 template <class T, class R, bool NORM>
 __global__ void __launch_bounds__(LONG_THREADS) long_rows_kernel(const __grid_constant__ Args a) {
@@ -454,7 +456,7 @@ void launch_block(const Args& a, cudaStream_t s) {
 }
 // Many rows: the smallest team whose registers hold a row at 32 values a thread (at 16 and 8 the instructions spent on
 // a row bind: 65536 x 4096 in bfloat16 took 441 us with 16, 303 us with 32), at 16 single values, whose registers
-// 32 do not fit. Few rows: 8 or 16 values a thread where all rows then run at once (1 x 4096: 2.6 us with 8, 3.8 us with
+// 32 do not fit. Few rows: 8 or 16 values a thread where all rows then run at once (1 x 4096: 2.5 us with 8, 3.8 us with
 // 32; 2000 x 1024: 4.5 us with 16, 5.7 us with 32; but 4000 x 1024: 8.3 and 6.9 us).
 template <class T, class R, Access A, bool NORM>
 void launch_rows(const Args& a, cudaStream_t s) {
@@ -585,7 +587,7 @@ __device__ __noinline__ uint32_t word_edge(const int8_t* p, const int8_t* first,
 // Rows at odd addresses or of odd groups: a thread takes the V values of an aligned
 // 32 bytes of output (the first and last piece of a row: of what the row has of
 // them) and gathers their bytes from aligned words. WALK: groups shorter than a piece.
-// Measured: 30000 x 7 x 333 bfloat16 values 97 us (2.15 TB/s; 238 us value by value),
+// Measured: 30000 x 7 x 333 bfloat16 values 96 us (2.18 TB/s; 238 us value by value),
 // bound by instructions.
 template <class T, bool WALK>
 __global__ void __launch_bounds__(256)
